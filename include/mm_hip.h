@@ -700,6 +700,59 @@ int mmh_bn_alice_prepare(const mmh_ctx *ctx, const uint64_t *d_rcm_r2f, const ui
 int mmh_bn_alice_finish(const mmh_ctx *ctx, const uint64_t *d_in_cts, const uint64_t *d_pts3, size_t n,
                         uint64_t *d_out_cts, void *stream);
 
+/* =====================================================================================
+ * Linear layers on shares without ciphertexts.  No counterpart in the reference, whose networks are convolutional: these
+ * are the pieces of a transformer layer that are linear with cleartext coefficients, so that a party computes them on its
+ * own share.
+ * ===================================================================================== */
+
+/* Products with cleartext weights, grouped by expert (what matVecMul computes under encryption, hom_fc_ss.cc:394-471, on ring
+ * words, for many rows and several weight matrices at once):
+ *   out[r][o] = add[r][o] + sum_k (x[t][k] + x1[t][k]) * w[g][o][k]  mod 2^ring_bw,  t = rows[r], offsets[g] <= r < offsets[g+1]
+ * The server runs it on inputs opened under a mask r whose ciphertext product W r - s ran ahead of the input
+ * (openmm_amd/ring_fc_ss.py): x = x0 - r from the client, x1 = its own share, add = s.  Which rows belong to which expert
+ * (or adapter, or client's model) is public.
+ *
+ * mmh_ring_weights_create lays out d_w [n_groups][rows][cols], contiguous signed integers of elem_bytes 1, 2, 4 or 8
+ * (ring elements: congruent modulo 2^ring_bw is the same weight), as byte digits in matrix-core order on the current
+ * device; weights need not be kept.  It reads the weights once to find how many digits the widest needs
+ * (mmh_ring_weights_info: `digits`), allocates and waits for the stream, so it fails under stream capture.  The handle is
+ * immutable: any number of streams and threads may use it, until destroy (which waits for kernels that read it). */
+typedef struct mmh_ring_weights mmh_ring_weights;
+int mmh_ring_weights_create(const void *d_w, int elem_bytes, size_t n_groups, size_t rows, size_t cols, int ring_bw,
+                            void *stream, mmh_ring_weights **out);
+int mmh_ring_weights_destroy(mmh_ring_weights *w);
+int mmh_ring_weights_info(const mmh_ring_weights *w, size_t *n_groups, size_t *rows, size_t *cols, int *ring_bw, int *digits);
+/* d_x [n_tokens] rows of cols words, ldx words apart; d_x1 (may be NULL) the same shape, ldx1 apart; any 64-bit words,
+ * taken mod 2^ring_bw.  d_rows [n_rows] (NULL: row r reads token r) may name a token any number of times; an index outside
+ * [0, n_tokens) reads as a row of zeros.  d_offsets [n_groups + 1], non-decreasing (NULL with one group: all rows); values
+ * are clamped to [0, n_rows] and output rows outside every group are left as they were.  d_add (may be NULL) n_rows rows
+ * ldadd apart (0: one row for all); it may be d_out with ldadd = ldo.  d_out must not overlap the other inputs.  Results
+ * are reduced mod 2^ring_bw and exact.  No workspace, no atomics: the call may be captured, and calls on different streams
+ * do not touch each other.  Runs on the weights' device.  n_rows <= 2^19 per call, n_groups <= 32767. */
+int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, size_t ldx, const uint64_t *d_x1, size_t ldx1,
+                    size_t n_tokens, const int64_t *d_rows, const int64_t *d_offsets, size_t n_rows, const uint64_t *d_add,
+                    size_t ldadd, uint64_t *d_out, size_t ldo, void *stream);
+
+/* Rotary positions on shares: in each head the pairs (a, b) of the first rot_dim words become
+ *   (a c - b s, b c + a s) mod 2^ring_bw,  c = round(amplitude 2^frac_bits cos(2 pi p f / 2^64)), s the same of the sine,
+ * with p = d_pos[token] (any 64-bit position) and f = d_phase[pair] the step as a fraction of a turn in units of 2^-64, so
+ * that p f mod 2^64 is exact at every position; the other words are multiplied by 2^frac_bits (one truncation then serves
+ * the whole head).  Pairs are (i, i + rot_dim/2), or (2i, 2i + 1) when interleaved.  The coefficients are a fixed sequence
+ * of IEEE double operations, rounded to the nearest integer, ties to even: two parties on this library get the same bits.
+ * x: word k of head h of token t at d_x[t*xs_token + h*xs_head + k]; out the same way with os_*, every row of its own
+ * (os_token, os_head >= head_dim where there is more than one).  d_out may be d_x with the same strides, else they must not
+ * overlap.  frac_bits <= 24, 0 < amplitude <= 16, head_dim <= 4096, n_heads <= 65536. */
+int mmh_rotary(const uint64_t *d_x, size_t xs_token, size_t xs_head, size_t n_tokens, size_t n_heads, size_t head_dim,
+               const int64_t *d_pos, const uint64_t *d_phase, size_t rot_dim, int interleaved, double amplitude, int frac_bits,
+               int ring_bw, uint64_t *d_out, size_t os_token, size_t os_head, void *stream);
+/* mmh_rotary followed by mmh_trunc_pre in one pass: d_adj [n_tokens][n_heads][head_dim] (and, unless NULL, d_cmp of the same
+ * shape, the operand of mill->compare) as mmh_trunc_pre would make them from the turned share (truncation-cheetah.cpp:23-56). */
+int mmh_rotary_trunc_pre(int party, const uint64_t *d_x, size_t xs_token, size_t xs_head, size_t n_tokens, size_t n_heads,
+                         size_t head_dim, const int64_t *d_pos, const uint64_t *d_phase, size_t rot_dim, int interleaved,
+                         double amplitude, int frac_bits, int ring_bw, int signed_arith, int heuristic, uint64_t *d_adj,
+                         uint64_t *d_cmp, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -214,7 +214,11 @@ class Truncation:
         adj, cmp = self._out(dim), self._out(dim)
         L.check(self.lib.mmh_trunc_pre(self.party, L.dptr(inA), dim, bw, int(signed_arithmetic), int(heuristic),
                                        L.dptr(adj), L.dptr(cmp), s))
-        wrap = wrap_of(L.to_host(adj), L.to_host(cmp))
+        return self._truncate_rest(dim, adj, cmp, shift, bw, signed_arithmetic, heuristic, wrap_of)
+
+    def _truncate_rest(self, dim, adj, cmp, shift, bw, signed_arithmetic, heuristic, wrap_of):
+        s = L._stream_ptr()
+        wrap = wrap_of(L.to_host(adj), None if cmp is None else L.to_host(cmp))
         aw = L.to_device(self.aux.B2A(self.party, wrap, dim, shift), f"cuda:{self.device}")
         out = self._out(dim)
         L.check(self.lib.mmh_trunc_post(self.party, L.dptr(adj), L.dptr(aw), dim, shift, bw,
@@ -230,6 +234,24 @@ class Truncation:
                                   lambda adj, cmp: self.aux.wrap(self.party, adj, dim, bw))
         return self._truncate(dim, inA, shift, bw, signed_arithmetic, False,
                               lambda adj, cmp: self.aux.compare(self.party, cmp, dim, bw))
+
+    def truncate_rotary(self, rotary, x, positions, shift, signed_arithmetic=True, apply_msb0_heuristic=True):
+        """truncate() of ``rotary.rotate(x, positions)``, [tokens, heads, head_dim], with the turn and the step before the
+        wrap protocol in one pass.  ``shift`` takes off the turn's frac_bits and whatever scale a product left in x."""
+        bw, dim = rotary.ring_bw, x.numel()
+        # what mmh_trunc_post asks for, before the protocol starts
+        if not (1 <= shift < bw and (not apply_msb0_heuristic or shift <= bw - 3)):
+            raise L.MMHError(7, "truncate_rotary: shift")
+        adj, cmp = rotary.truncate_pre(self.party, x, positions, signed_arithmetic, apply_msb0_heuristic)
+        if dim == 0:
+            return adj
+        if apply_msb0_heuristic:
+            wrap_of = lambda a, c: self.aux.wrap(self.party, a, dim, bw)
+        else:
+            wrap_of = lambda a, c: self.aux.compare(self.party, c, dim, bw)
+        flat = None if cmp is None else cmp.view(-1)
+        out = self._truncate_rest(dim, adj.view(-1), flat, shift, bw, signed_arithmetic, apply_msb0_heuristic, wrap_of)
+        return out.view(x.shape)
 
     # :84-151 (the sub-protocol gets msb_x, inverted on ALICE when signed, :118-127; the ideal one ignores it)
     def truncate_msb(self, dim, inA, shift, bw, signed_arithmetic, msb_x):
