@@ -6,7 +6,7 @@
 // digit + 128, the exclusive or takes the 128 off again as a signed byte).  l bits need nx = ceil(l/8) digits of x (what
 // lies above is a multiple of 2^l), a weight as many as its size asks for, found when the weights are laid out.  The
 // product modulo 2^l is then sum over s < nx of 256^s * sum_{i+j=s} x_i w_j, every inner sum an exact i8 x i8 -> i32
-// matrix product (v_mfma_i32_16x16x64_i8), nx accumulators per output.  |x_i w_j| <= 2^14 and at most nw products share
+// matrix product (v_mfma_i32_32x32x32_i8, 1.6 times the rate of the 16x16x64 form), nx accumulators per output.  |x_i w_j| <= 2^14 and at most nw products share
 // an accumulator, so up to (2^17 - 1) / nw terms of k cannot overflow; longer k is added up in 64-bit pieces.
 // Everything is exact: the result does not depend on the order of the sums.
 #include <algorithm>
@@ -19,22 +19,23 @@ struct mmh_ring_weights {
   int device = 0;
   size_t groups = 0, rows = 0, cols = 0;
   int bw = 0, nx = 0, nw = 0;   // nw: digits stored per weight (a width the product kernels exist for)
-  size_t k64 = 0, out16 = 0;
-  int8_t *d = nullptr;          // [group][out16][k64][digit][4][16 outputs][16 columns]: 1 KiB matrix-core fragments
+  size_t k32 = 0, out32 = 0;    // fragments along the columns (an even number) and the outputs
+  int8_t *d = nullptr;          // [group][out32][k32][digit][2][32 outputs][16 columns]: 1 KiB matrix-core fragments
 };
 
 namespace mmh {
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
 
 struct RingArgs {
   const int8_t *w;
   const u64 *x, *x1, *add;
   const int64_t *rows, *offsets;
-  u64 *out;
+  u64 *out, *ws;               // ws: where the parts of k go that ring_join_kernel adds up (null: straight to out)
   size_t ldx, ldx1, ldadd, ldo, n_tokens, n_rows;
-  int groups, cols, n_out, k64, out16;
+  int groups, cols, n_out, k32, out32, out_tiles, row_tiles;
   u64 mask;
-  int vec_x, vec_out;   // 16-byte accesses are aligned
+  int zero_rest;
 };
 
 // The rows of row tile `tile` (BM rows, tiles do not cross groups).  Every wave finds it by itself: 64 groups at a time,
@@ -78,21 +79,52 @@ __device__ __forceinline__ bool ring_find_tile(const RingArgs &a, u32 tile, int 
   return false;
 }
 
+// Which tile a workgroup computes.  Workgroups go round the 8 XCDs, each with an L2 of its own, so every XCD gets a contiguous
+// piece of the order "four output tiles across, row tiles down": the workgroups that run there at one time share rows and
+// weights.
+__device__ __forceinline__ bool ring_block(const RingArgs &a, int &ot, int &rt) {
+  // with eight row tiles or more an XCD takes every eighth of them, so that tiles no group has are spread evenly
+  const bool deal = a.row_tiles >= 8;
+  const u32 rows = deal ? (a.row_tiles + 7) / 8 : a.row_tiles, total = (u32)a.out_tiles * rows, per = deal ? total : (total + 7) / 8;
+  const u32 q = (deal ? 0 : (blockIdx.x & 7) * per) + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || q >= total) return false;
+  const u32 panel = q / (4 * rows), rest = q - panel * 4 * rows;
+  const u32 wide = (u32)a.out_tiles - panel * 4 < 4 ? (u32)a.out_tiles - panel * 4 : 4;
+  rt = (int)(rest / wide), ot = (int)(panel * 4 + rest % wide);
+  if (deal) rt = rt * 8 + (int)(blockIdx.x & 7);
+  return rt < a.row_tiles;
+}
+
 // the row of x that row r reads, or -1 (an index outside [0, n_tokens) reads as a row of zeros)
 __device__ __forceinline__ long long ring_token(const RingArgs &a, size_t r) {
   const long long t = a.rows ? a.rows[r] : (long long)r;
   return t >= 0 && t < (long long)a.n_tokens ? t : -1;
 }
 
-// four words of a row from column k on (zeros past the end), plus the second share's
-__device__ __forceinline__ void ring_load4(const u64 *p, int k, int cols, int vec, u64 (&v)[4]) {
-  if (vec && k + 4 <= cols) {
-    const ulonglong2 t = *reinterpret_cast<const ulonglong2 *>(p + k), u = *reinterpret_cast<const ulonglong2 *>(p + k + 2);
-    v[0] = t.x, v[1] = t.y, v[2] = u.x, v[3] = u.y;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = k + e < cols ? p[k + e] : 0;
+// rows that no group has, in the columns [n0, n1): zeros, where the caller asked for them
+__device__ __forceinline__ void ring_zero_rest(const RingArgs &a, int n0, int n1) {
+  if (!a.zero_rest || !a.offsets) return;
+  const long long n = (long long)a.n_rows;
+  long long b = a.offsets[0], e = a.offsets[a.groups];
+  b = b < 0 ? 0 : b > n ? n : b, e = e < b ? b : e > n ? n : e;
+  n1 = n1 < a.n_out ? n1 : a.n_out;
+  for (long long row = 0; row < n; ++row) {
+    if (row == b) row = e;
+    if (row >= n) break;
+    for (int i = n0 + (int)threadIdx.x; i < n1; i += blockDim.x) a.out[(size_t)row * a.ldo + i] = 0;
   }
+}
+
+struct __attribute__((packed, aligned(8))) Words2 {   // 16-byte accesses to 8-byte aligned words
+  u64 v[2];
+};
+__device__ __forceinline__ void ring_load4(const u64 *p, u64 (&v)[4]) {
+  const Words2 t = reinterpret_cast<const Words2 *>(p)[0], u = reinterpret_cast<const Words2 *>(p)[1];
+  v[0] = t.v[0], v[1] = t.v[1], v[2] = u.v[0], v[3] = u.v[1];
+}
+__device__ __forceinline__ void ring_store4(u64 *p, const u64 (&v)[4]) {
+  reinterpret_cast<Words2 *>(p)[0] = Words2{{v[0], v[1]}};
+  reinterpret_cast<Words2 *>(p)[1] = Words2{{v[2], v[3]}};
 }
 // bytes e[0..3].b -> one dword per byte place: a 4 x 4 byte transposition
 __device__ __forceinline__ void transpose4(u32 e0, u32 e1, u32 e2, u32 e3, u32 (&d)[4]) {
@@ -101,13 +133,13 @@ __device__ __forceinline__ void transpose4(u32 e0, u32 e1, u32 e2, u32 e3, u32 (
   d[0] = __builtin_amdgcn_perm(l1, l0, 0x05040100), d[1] = __builtin_amdgcn_perm(l1, l0, 0x07060302);
   d[2] = __builtin_amdgcn_perm(h1, h0, 0x05040100), d[3] = __builtin_amdgcn_perm(h1, h0, 0x07060302);
 }
+constexpr u64 kDigitBias = 0x8080808080808080ull;
 // digits of four words: dig[i] holds digit i of each
 template <int NX>
 __device__ __forceinline__ void ring_digits4(const u64 (&v)[4], u32 (&dig)[8]) {
-  constexpr u64 C = 0x8080808080808080ull;
   u64 t[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) t[e] = v[e] + C;
+  for (int e = 0; e < 4; ++e) t[e] = v[e] + kDigitBias;
   u32 d[4];
   transpose4(lo32(t[0]), lo32(t[1]), lo32(t[2]), lo32(t[3]), d);
 #pragma unroll
@@ -119,229 +151,275 @@ __device__ __forceinline__ void ring_digits4(const u64 (&v)[4], u32 (&dig)[8]) {
   }
 }
 
-// Few rows: one workgroup per 16 rows x 16*OT outputs, its WK waves split k and join their 64-bit sums through LDS.
-// Bound: the weights' bytes.  A lane reads the 16 words of its fragment itself and cuts them to digits in registers, so
-// the loop has no LDS access and no barrier.
-template <int NX, int NW, int OT, int WK>
-__global__ __launch_bounds__(64 * WK) void ring_rows_kernel(RingArgs a) {
-  __shared__ u64 part[WK][OT][16][17];
+// ---- the rows' digits.  A lane cuts four words of one row: block b of a step is 16 rows (b & 1 ...) x 16 columns, and in it
+// lane l takes row l % 16, columns 4 * (l / 16) ..; four lanes read 128 contiguous bytes, and the 64 dwords a block gives per
+// digit fall into 64 different LDS banks.
+struct RingRow {
+  const u64 *x, *x1;   // null: a row of zeros
+};
+__device__ __forceinline__ RingRow ring_row(const RingArgs &a, size_t row, size_t hi) {
+  const long long t = row < hi ? ring_token(a, row) : -1;
+  return RingRow{t < 0 ? nullptr : a.x + (size_t)t * a.ldx, t < 0 || !a.x1 ? nullptr : a.x1 + (size_t)t * a.ldx1};
+}
+__device__ __forceinline__ void ring_load_row(const RingArgs &a, const RingRow &p, int k, u64 (&v)[4], u64 (&u)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = 0, u[e] = 0;
+  if (k + 4 <= a.cols) {
+    if (p.x) ring_load4(p.x + k, v);
+    if (p.x1) ring_load4(p.x1 + k, u);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (p.x && k + e < a.cols) v[e] = p.x[k + e];
+      if (p.x1 && k + e < a.cols) u[e] = p.x1[k + e];
+    }
+  }
+}
+// into the fragment of each digit: lane (k / 16) * 32 + row holds 16 columns of a row; frag points at digit 0's
+template <int NX>
+__device__ __forceinline__ void ring_store_digits(uint4 *frag, int row, int k16, int sub, const u64 (&v)[4], const u64 (&u)[4]) {
+  u64 t[4];
+  u32 dig[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) t[e] = v[e] + u[e];
+  ring_digits4<NX>(t, dig);
+#pragma unroll
+  for (int d = 0; d < NX; ++d) reinterpret_cast<u32 *>(&frag[d * 64 + k16 * 32 + row])[sub] = dig[d];
+}
+__device__ __forceinline__ v4i as_v4i(const uint4 &t) { return v4i{(int)t.x, (int)t.y, (int)t.z, (int)t.w}; }
+// the 64-bit value of element e of a 32 x 32 tile from its digit sums
+template <int NX>
+__device__ __forceinline__ u64 ring_value(const v16i (&acc)[NX], int e) {
+  u64 v = 0;
+#pragma unroll
+  for (int s = NX - 1; s >= 0; --s) v = (v << 8) + (u64)(long long)acc[s][e];
+  return v;
+}
+
+// first column of fragment c: steps of two fragments, the last of which ends with the last column (weights of columns that the
+// step before has already are laid out as zeros)
+__device__ __forceinline__ int ring_column(const RingArgs &a, int c) {
+  const int k = (c >> 1) * 64;
+  return (c >> 1) == a.k32 / 2 - 1 && a.cols > 64 ? a.cols - 64 + (c & 1) * 32 : k + (c & 1) * 32;
+}
+
+// Small products: one workgroup per 32 rows x 32 outputs, its WK waves split k in steps of 32 columns and join their 64-bit
+// sums through LDS.  Every wave cuts its own digits into LDS of its own, so the loop has no barrier.
+template <int NX, int NW, int WK>
+__global__ __launch_bounds__(64 * WK, 2) void ring_rows_kernel(RingArgs a) {
+  __shared__ uint4 lds[WK][512];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   int g;
   size_t lo, hi;
-  if (!ring_find_tile<16>(a, blockIdx.y, g, lo, hi)) return;
-  const int ot0 = (int)blockIdx.x * OT, r = lane & 15, kq = lane >> 4;
-  const long long t = lo + r < hi ? ring_token(a, lo + r) : -1;
-  const u64 *px = t < 0 ? nullptr : a.x + (size_t)t * a.ldx;
-  const u64 *px1 = t < 0 || !a.x1 ? nullptr : a.x1 + (size_t)t * a.ldx1;
-  constexpr int kFlush = 131071 / NW / 64;   // chunks whose sums fit 32 bits
-  u64 total[OT][4] = {};
-  v4i acc[OT][NX];
+  if (blockIdx.y == 0) ring_zero_rest(a, (int)blockIdx.x * 32, (int)blockIdx.x * 32 + 32);
+  if (!ring_find_tile<32>(a, blockIdx.y, g, lo, hi)) return;
+  const int ot = (int)blockIdx.x, r = lane & 15, sub = lane >> 4;
+  const RingRow row[2] = {ring_row(a, lo + r, hi), ring_row(a, lo + 16 + r, hi)};
+  const int8_t *pw = a.w + ((size_t)g * a.out32 + ot) * a.k32 * (NW * 1024) + lane * 16;
+  v16i acc[NX];
 #pragma unroll
-  for (int o = 0; o < OT; ++o)
+  for (int s = 0; s < NX; ++s)
 #pragma unroll
-    for (int s = 0; s < NX; ++s) acc[o][s] = v4i{0, 0, 0, 0};
-  auto fold = [&] {
+    for (int e = 0; e < 16; ++e) acc[s][e] = 0;
+  u64 xv[4][4], xu[4][4];
+  v4i w[NW];
+  auto load = [&](int c) {
 #pragma unroll
-    for (int o = 0; o < OT; ++o) {
+    for (int j = 0; j < NW; ++j) w[j] = *reinterpret_cast<const v4i *>(pw + ((size_t)c * NW + j) * 1024);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        u64 v = 0;
-#pragma unroll
-        for (int s = NX - 1; s >= 0; --s) v = (v << 8) + (u64)(long long)acc[o][s][e];
-        total[o][e] += v;
-      }
-#pragma unroll
-      for (int s = 0; s < NX; ++s) acc[o][s] = v4i{0, 0, 0, 0};
-    }
+    for (int b = 0; b < 4; ++b) ring_load_row(a, row[b & 1], ring_column(a, c) + (b >> 1) * 16 + sub * 4, xv[b], xu[b]);
   };
-  int since = 0;
-  for (int c = wave; c < a.k64; c += WK) {
-    v4i w[OT][NW];
+  if (wave < a.k32) load(wave);
+  for (int c = wave; c < a.k32; c += WK) {
 #pragma unroll
-    for (int o = 0; o < OT; ++o) {
-      const int ot = ot0 + o < a.out16 ? ot0 + o : a.out16 - 1;
-      const int8_t *p = a.w + (((size_t)g * a.out16 + ot) * a.k64 + c) * (NW * 1024) + lane * 16;
+    for (int b = 0; b < 4; ++b) ring_store_digits<NX>(lds[wave], (b & 1) * 16 + r, b >> 1, sub, xv[b], xu[b]);
+    v4i wc[NW];
 #pragma unroll
-      for (int j = 0; j < NW; ++j) w[o][j] = *reinterpret_cast<const v4i *>(p + j * 1024);
-    }
-    u64 v[4][4] = {};
-    if (px) {
-      const int k = c * 64 + kq * 16;
+    for (int j = 0; j < NW; ++j) wc[j] = w[j];
+    if (c + WK < a.k32) load(c + WK);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ring_load4(px, k + 4 * e, a.cols, a.vec_x, v[e]);
-      if (px1) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          u64 u[4];
-          ring_load4(px1, k + 4 * e, a.cols, a.vec_x, u);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[e][i] += u[i];
-        }
-      }
-    }
-    v4i x[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      u32 dig[8];
-      ring_digits4<NX>(v[e], dig);
-#pragma unroll
-      for (int i = 0; i < NX; ++i) x[i][e] = (int)dig[i];
-    }
-#pragma unroll
-    for (int o = 0; o < OT; ++o)
+    for (int i = 0; i < NX; ++i) {
+      const v4i x = as_v4i(lds[wave][i * 64 + lane]);
 #pragma unroll
       for (int j = 0; j < NW; ++j)
-#pragma unroll
-        for (int i = 0; i < NX; ++i)
-          if (i + j < NX) acc[o][i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[o][j], x[i], acc[o][i + j], 0, 0, 0);
-    if (++since == kFlush) fold(), since = 0;
+        if (i + j < NX) acc[i + j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wc[j], x, acc[i + j], 0, 0, 0);
+    }
   }
-  fold();
-  // a lane holds outputs 4*(lane/16) .. +3 of row lane%16
+  // element e of a lane: row lane % 32, output e % 4 + 8 * (e / 4) + 4 * (lane / 32)
+  u64 *part = reinterpret_cast<u64 *>(lds[wave]);
 #pragma unroll
-  for (int o = 0; o < OT; ++o)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) part[wave][o][r][kq * 4 + e] = total[o][e];
+  for (int e = 0; e < 16; ++e) part[e * 64 + lane] = ring_value<NX>(acc, e);
   __syncthreads();
-  for (int i = (int)threadIdx.x; i < OT * 256; i += 64 * WK) {
-    const int col = i & 15, o = (i >> 4) % OT, row = i / (16 * OT);
-    const int n = (ot0 + o) * 16 + col;
-    if (lo + row >= hi || n >= a.n_out) continue;
-    u64 v = a.add ? a.add[(lo + row) * a.ldadd + n] : 0;
+  for (int i = (int)threadIdx.x; i < 1024; i += 64 * WK) {
+    const int o = i & 31, rr = i >> 5, n = ot * 32 + o;
+    if (lo + rr >= hi || n >= a.n_out) continue;
+    const int at = ((o & 3) + 4 * (o >> 3)) * 64 + (o >> 2 & 1) * 32 + rr;
+    u64 v = a.add ? a.add[(lo + rr) * a.ldadd + n] : 0;
 #pragma unroll
-    for (int w = 0; w < WK; ++w) v += part[w][o][row][col];
-    a.out[(lo + row) * a.ldo + n] = v & a.mask;
+    for (int k = 0; k < WK; ++k) v += reinterpret_cast<const u64 *>(lds[k])[at];
+    a.out[(lo + rr) * a.ldo + n] = v & a.mask;
   }
 }
 
-// Many rows: a workgroup of WR x WO waves computes 16*RT*WR rows x 16*OT*WO outputs.  The rows' digits of one 64-column
-// step are cut once per workgroup into LDS (two buffers, one barrier per step); the weights' fragments come straight from
-// L2 in the order they were laid out in.
-template <int NX, int NW, int RT, int OT, int WR, int WO>
-__global__ __launch_bounds__(64 * WR * WO) void ring_tile_kernel(RingArgs a) {
-  constexpr int BM = 16 * RT * WR, W = WR * WO, kBlocks = BM / 16 * 4, kPer = (kBlocks + W - 1) / W;
-  static_assert(kBlocks % W == 0, "every wave cuts the same number of 16 x 16 blocks");
-  __shared__ uint4 xs[2][BM / 16][NX][64];
+// Large products: a workgroup of 8 waves computes 32 rows x 256*OT outputs in steps of 64 columns.  The rows' digits are cut
+// once per workgroup into LDS (three buffers, one barrier per step); the weights' fragments come straight from L2 in the order
+// they were laid out in.  Words and weights are loaded into registers two steps before they are used; nothing in the loop
+// branches.  Needs 64 columns or more.
+template <int NX, int NW, int OT, bool TWO>
+__global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
+  __shared__ uint4 xs[3][2 * NX * 64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  int g;
+  int g, ot, rt;
   size_t lo, hi;
-  if (!ring_find_tile<BM>(a, blockIdx.y, g, lo, hi)) return;
-  const int wr = wave % WR, wo = wave / WR, ot0 = ((int)blockIdx.x * WO + wo) * OT;
+  if (!ring_block(a, ot, rt)) return;
+  if (rt == 0 && !a.ws) ring_zero_rest(a, ot * 256 * OT, (ot + 1) * 256 * OT);
+  if (!ring_find_tile<32>(a, rt, g, lo, hi)) return;
+  const int ot0 = (ot * 8 + wave) * OT;
   const int r = lane & 15, sub = lane >> 4;
-  // block b of the step: row tile b / 4, columns 16 * (b % 4) ..; a lane cuts four words of one row
-  const u64 *px[kPer], *px1[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const size_t row = lo + (size_t)((i * W + wave) / 4) * 16 + r;
-    const long long t = row < hi ? ring_token(a, row) : -1;
-    px[i] = t < 0 ? nullptr : a.x + (size_t)t * a.ldx;
-    px1[i] = t < 0 || !a.x1 ? nullptr : a.x1 + (size_t)t * a.ldx1;
-  }
-  u64 xv[kPer][4], xu[kPer][4];
-  auto load_x = [&](int c) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int k = c * 64 + ((i * W + wave) & 3) * 16 + sub * 4;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) xv[i][e] = 0, xu[i][e] = 0;
-      if (px[i]) ring_load4(px[i], k, a.cols, a.vec_x, xv[i]);
-      if (px1[i]) ring_load4(px1[i], k, a.cols, a.vec_x, xu[i]);
-    }
+  // this wave cuts the 16 x 16 block (row half wave % 2, column quarter wave / 2) of every step
+  const size_t my_row = lo + (wave & 1) * 16 + r;
+  const long long my_token = my_row < hi ? ring_token(a, my_row) : -1;
+  const size_t token = my_token < 0 ? 0 : (size_t)my_token;   // any row will do: its sums are not used
+  const int in_step = (wave >> 1) * 16 + sub * 4;
+  const u64 *px = a.x + token * a.ldx + in_step, *px1 = TWO ? a.x1 + token * a.ldx1 + in_step : nullptr;
+  u64 xv[2][4], xu[2][4];
+  const int last = a.k32 / 2 - 1;
+  auto load_x = [&](int p, int c) {
+    c = c < last ? c : last;
+    const int k = c * 64 < a.cols - 64 ? c * 64 : a.cols - 64;   // the last step ends with the last column
+    ring_load4(px + k, xv[p]);
+    if (TWO) ring_load4(px1 + k, xu[p]);
   };
-  auto store_x = [&](int buf) {
+  // half 0: digits 0 .. 3, half 1: the others
+  auto store_x = [&](int p, int buf, int half) {
+    u32 d[4];
+    u64 t[4];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int b = i * W + wave;
-      u64 v[4];
-      u32 dig[8];
+    for (int e = 0; e < 4; ++e) t[e] = (TWO ? xv[p][e] + xu[p][e] : xv[p][e]) + kDigitBias;
+    if (half == 0) transpose4(lo32(t[0]), lo32(t[1]), lo32(t[2]), lo32(t[3]), d);
+    else transpose4(hi32(t[0]), hi32(t[1]), hi32(t[2]), hi32(t[3]), d);
+    uint4 *frag = xs[buf] + (wave >> 2) * (NX * 64) + (wave >> 1 & 1) * 32 + (wave & 1) * 16 + r;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = xv[i][e] + xu[i][e];
-      ring_digits4<NX>(v, dig);
-#pragma unroll
-      for (int d = 0; d < NX; ++d) reinterpret_cast<u32 *>(&xs[buf][b >> 2][d][(b & 3) * 16 + r])[sub] = dig[d];
-    }
+    for (int k = 0; k < 4; ++k)
+      if (4 * half + k < NX) reinterpret_cast<u32 *>(frag + (4 * half + k) * 64)[sub] = d[k] ^ lo32(kDigitBias);
   };
   const int8_t *pw[OT];
 #pragma unroll
   for (int o = 0; o < OT; ++o) {
-    const int ot = ot0 + o < a.out16 ? ot0 + o : a.out16 - 1;
-    pw[o] = a.w + ((size_t)g * a.out16 + ot) * a.k64 * (NW * 1024) + lane * 16;
+    const int t = ot0 + o < a.out32 ? ot0 + o : a.out32 - 1;
+    pw[o] = a.w + ((size_t)g * a.out32 + t) * a.k32 * (NW * 1024);
   }
-  v4i wn[OT][NW], wc[OT][NW], acc[RT][OT][NX];
-  auto load_w = [&](int c) {
+  v4i w[2][2][OT][NW];
+  v16i acc[OT][NX];
+  auto load_w = [&](int p, int h, int c) {
+    c = c < last ? c : last;
 #pragma unroll
     for (int o = 0; o < OT; ++o)
 #pragma unroll
-      for (int j = 0; j < NW; ++j) wn[o][j] = *reinterpret_cast<const v4i *>(pw[o] + (size_t)c * (NW * 1024) + j * 1024);
+      for (int j = 0; j < NW; ++j) w[p][h][o][j] = reinterpret_cast<const v4i *>(pw[o] + ((size_t)(2 * c + h) * NW + j) * 1024)[lane];
   };
-  constexpr int kFlush = 131071 / NW / 64;
-  for (int c0 = 0; c0 < a.k64; c0 += kFlush) {
-    const int c1 = c0 + kFlush < a.k64 ? c0 + kFlush : a.k64;
+  // fragment t of a step (column half t / NX, digit t % NX) is read from LDS D products' places ahead of its use
+  constexpr int D = NX == 5 ? 4 : 3;
+  static_assert(2 * NX % (D + 1) == 0, "a step leaves the ring of fragments where it found it");
+  v4i f[D + 1];
+  // the barrier orders LDS alone: loads from memory stay in flight across it
+  auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  // Step c (p = c % 2): products from buffer rd, digits of step c + 2 into wr.  The barrier in its middle publishes them; the
+  // buffer they replace was read a step ago, before that step's barrier or right after it, never behind this one.
+  constexpr int kCut = NX <= 5 ? 1 : NX - 4;
+  int rd = 0, nx = 1, wr = 2;
+  // Products, reads and the cutting of digits are kept in this order (sched_barrier): moved together, the cutting would wait
+  // for words that were only just asked for, and reads for products.
+  auto step = [&](int p, int c) {
 #pragma unroll
-    for (int m = 0; m < RT; ++m)
+    for (int t = 0; t < 2 * NX; ++t) {
+      const int n = t + D, i = t % NX, h = t / NX;
+      f[n % (D + 1)] = as_v4i(n < 2 * NX ? xs[rd][n * 64 + lane] : xs[nx][(n - 2 * NX) * 64 + lane]);
 #pragma unroll
       for (int o = 0; o < OT; ++o)
 #pragma unroll
-        for (int s = 0; s < NX; ++s) acc[m][o][s] = v4i{0, 0, 0, 0};
-    load_x(c0);
-    load_w(c0);
-    store_x(0);
-    __syncthreads();
-    int buf = 0;
-    for (int c = c0; c < c1; ++c) {
-#pragma unroll
-      for (int o = 0; o < OT; ++o)
-#pragma unroll
-        for (int j = 0; j < NW; ++j) wc[o][j] = wn[o][j];
-      const bool more = c + 1 < c1;
-      if (more) load_x(c + 1), load_w(c + 1);
-#pragma unroll
-      for (int m = 0; m < RT; ++m)
-#pragma unroll
-        for (int i = 0; i < NX; ++i) {
-          const uint4 t = xs[buf][wr * RT + m][i][lane];
-          const v4i x = v4i{(int)t.x, (int)t.y, (int)t.z, (int)t.w};
-#pragma unroll
-          for (int o = 0; o < OT; ++o)
-#pragma unroll
-            for (int j = 0; j < NW; ++j)
-              if (i + j < NX)
-                acc[m][o][i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wc[o][j], x, acc[m][o][i + j], 0, 0, 0);
-        }
-      if (more) store_x(buf ^ 1);
-      __syncthreads();
-      buf ^= 1;
-    }
-    // a lane holds outputs 4*(lane/16) .. +3 of row lane%16 of each tile
-#pragma unroll
-    for (int m = 0; m < RT; ++m) {
-      const size_t row = lo + (size_t)(wr * RT + m) * 16 + r;
-      if (row >= hi) continue;
-      const u64 *base = c0 ? a.out + row * a.ldo : a.add ? a.add + row * a.ldadd : nullptr;
-#pragma unroll
-      for (int o = 0; o < OT; ++o) {
-        const int n = (ot0 + o) * 16 + sub * 4;
-        u64 v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = 0;
-#pragma unroll
-          for (int s = NX - 1; s >= 0; --s) v[e] = (v[e] << 8) + (u64)(long long)acc[m][o][s][e];
-          if (base && n + e < a.n_out) v[e] += base[n + e];
-          v[e] &= a.mask;
-        }
-        u64 *p = a.out + row * a.ldo + n;
-        if (a.vec_out && n + 4 <= a.n_out) {
-          reinterpret_cast<ulonglong2 *>(p)[0] = make_ulonglong2(v[0], v[1]);
-          reinterpret_cast<ulonglong2 *>(p)[1] = make_ulonglong2(v[2], v[3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < a.n_out) p[e] = v[e];
-        }
+        for (int j = 0; j < NW; ++j)
+          if (i + j < NX)
+            acc[o][i + j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[p][h][o][j], f[t % (D + 1)], acc[o][i + j], 0, 0, 0);
+      if (t == kCut) store_x(p, wr, 0);
+      if (NX > 4 && t == kCut + 2) store_x(p, wr, 1);
+      if (t == NX - 1) {
+        load_x(p, c + 4);
+        load_w(p, 0, c + 2);
+        barrier();
       }
+      __builtin_amdgcn_sched_barrier(0x4);   // scalar arithmetic may cross
+    }
+    load_w(p, 1, c + 2);
+    const int t = rd;
+    rd = nx, nx = wr, wr = t;
+    __builtin_amdgcn_sched_barrier(0x4);
+  };
+  constexpr int kFlush = 131071 / NW / 64;   // steps whose sums fit 32 bits
+  const int first = (int)((long long)(last + 1) * blockIdx.y / gridDim.y);
+  const int end = (int)((long long)(last + 1) * (blockIdx.y + 1) / gridDim.y);
+  for (int c0 = first; c0 < end; c0 += kFlush) {
+    const int c1 = c0 + kFlush < end ? c0 + kFlush : end;
+#pragma unroll
+    for (int o = 0; o < OT; ++o)
+#pragma unroll
+      for (int s = 0; s < NX; ++s)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[o][s][e] = 0;
+    load_x(0, c0);
+    load_x(1, c0 + 1);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) load_w(p, 0, c0 + p), load_w(p, 1, c0 + p);
+#pragma unroll
+    for (int half = 0; half < (NX > 4 ? 2 : 1); ++half) store_x(0, rd, half), store_x(1, nx, half);
+    load_x(0, c0 + 2);
+    load_x(1, c0 + 3);
+    barrier();
+#pragma unroll
+    for (int t = 0; t < D; ++t) f[t] = as_v4i(xs[rd][t * 64 + lane]);
+    int c = c0;
+    for (; c + 1 < c1; c += 2) step(0, c), step(1, c + 1);
+    if (c < c1) step(0, c);
+    // element e of a lane: row lane % 32, output e % 4 + 8 * (e / 4) + 4 * (lane / 32)
+    const size_t row = lo + (lane & 31);
+    if (row < hi) {
+      const bool none = ring_token(a, row) < 0;
+      u64 *dst = a.ws ? a.ws + ((size_t)blockIdx.y * a.n_rows + row) * a.n_out : a.out + row * a.ldo;
+      const u64 *base = c0 > first ? dst : a.add && !a.ws ? a.add + row * a.ldadd : nullptr;
+#pragma unroll
+      for (int o = 0; o < OT; ++o)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = (ot0 + o) * 32 + q * 8 + (lane >> 5) * 4;
+          u64 v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = none ? 0 : ring_value<NX>(acc[o], q * 4 + e);
+            if (base && n + e < a.n_out) v[e] += base[n + e];
+            v[e] &= a.mask;
+          }
+          if (n + 4 <= a.n_out) ring_store4(dst + n, v);
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < a.n_out) dst[n + e] = v[e];
+        }
     }
   }
+}
+
+// the parts of k that several workgroups summed: out = add + sum of the parts
+__global__ __launch_bounds__(256) void ring_join_kernel(RingArgs a, int parts) {
+  const int n = (int)(blockIdx.x * 256 + threadIdx.x);
+  const size_t row = blockIdx.y;
+  if (n >= a.n_out) return;
+  if (a.offsets && ((long long)row < a.offsets[0] || (long long)row >= a.offsets[a.groups])) {
+    if (a.zero_rest) a.out[row * a.ldo + n] = 0;
+    return;
+  }
+  u64 v = a.add ? a.add[row * a.ldadd + n] : 0;
+  for (int p = 0; p < parts; ++p) v += a.ws[((size_t)p * a.n_rows + row) * a.n_out + n];
+  a.out[row * a.ldo + n] = v & a.mask;
 }
 
 // ---- weights: how many digits the widest needs, then the layout
@@ -364,16 +442,18 @@ __global__ __launch_bounds__(256) void ring_weight_digits_kernel(const T *__rest
 }
 template <typename T>
 __global__ __launch_bounds__(256) void ring_weight_layout_kernel(const T *__restrict__ w, size_t rows, size_t cols, int bw,
-                                                                 size_t out16, size_t k64, int nw, size_t n_units,
+                                                                 size_t out32, size_t k32, int nw, size_t n_units,
                                                                  int8_t *__restrict__ out) {
-  const size_t u = (size_t)blockIdx.x * 256 + threadIdx.x;   // (group, out16, k64, quarter, output): 16 columns of a row
+  const size_t u = (size_t)blockIdx.x * 256 + threadIdx.x;   // (group, out32, k32, half, output): 16 columns of a row
   if (u >= n_units) return;
-  const size_t frag = u >> 6, c = frag % k64, ot = frag / k64 % out16, g = frag / k64 / out16;
-  const size_t o = ot * 16 + (u & 15), k = c * 64 + (u >> 4 & 3) * 16;
+  const size_t frag = u >> 6, c = frag % k32, ot = frag / k32 % out32, g = frag / k32 / out32;
+  // columns as ring_column has them: the last step of 64 ends with the last column and skips what the step before has
+  const size_t step = c >> 1, start = step == k32 / 2 - 1 && cols > 64 ? cols - 64 : step * 64;
+  const size_t o = ot * 32 + (u & 31), k = start + (c & 1) * 32 + (u >> 5 & 1) * 16;
   u64 t[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const bool in = o < rows && k + e < cols;
+    const bool in = o < rows && k + e < cols && k + e >= step * 64;
     const u64 C = 0x8080808080808080ull;
     t[e] = ((u64)(in ? ring_weight(w, (g * rows + o) * cols + k + e, bw) : 0) + C) ^ C;
   }
@@ -392,24 +472,36 @@ static void ring_launch_digits(const void *w, size_t n, int bw, int *need, hipSt
 }
 template <typename T>
 static void ring_launch_layout(const void *w, const mmh_ring_weights *h, hipStream_t s) {
-  const size_t units = h->groups * h->out16 * h->k64 * 64;
+  const size_t units = h->groups * h->out32 * h->k32 * 64;
   hipLaunchKernelGGL(ring_weight_layout_kernel<T>, dim3((unsigned)((units + 255) / 256)), dim3(256), 0, s, (const T *)w,
-                     h->rows, h->cols, h->bw, h->out16, h->k64, h->nw, units, h->d);
+                     h->rows, h->cols, h->bw, h->out32, h->k32, h->nw, units, h->d);
 }
 
+// parts of k for `tiles` workgroups of the tile kernel: fill the chip's 256 compute units, four steps or more each
+static int ring_parts(size_t tiles, size_t steps) {
+  return (int)std::max<size_t>(1, std::min(std::min<size_t>(256 / std::max<size_t>(tiles, 1), steps / 4), size_t(16)));
+}
+// 32-output tiles a wave computes: the accumulators of one take 16 nx registers; two while they fit, for fewer digit reads
+static constexpr int ring_outputs(int nx, int nw) { return nx * 32 + nw * 32 <= 160 ? 2 : 1; }
+
 template <int NX, int NW>
-static void ring_launch(const RingArgs &a, hipStream_t s) {
-  // row tiles of BM rows that the groups can have: each nonempty group has at most one that is not full
-  auto tiles = [&](size_t bm) { return a.offsets ? a.n_rows / bm + std::min<size_t>((size_t)a.groups, a.n_rows) : (a.n_rows + bm - 1) / bm; };
-  if (a.n_rows <= 16 * (size_t)a.groups) {
-    constexpr int OT = 1, WK = 8;
-    hipLaunchKernelGGL((ring_rows_kernel<NX, NW, OT, WK>), dim3((a.out16 + OT - 1) / OT, (unsigned)tiles(16)), dim3(64 * WK),
-                       0, s, a);
-  } else {
-    constexpr int RT = 2, OT = 2, WR = 1, WO = 4;
-    hipLaunchKernelGGL((ring_tile_kernel<NX, NW, RT, OT, WR, WO>),
-                       dim3((a.out16 + OT * WO - 1) / (OT * WO), (unsigned)tiles(16 * RT * WR)), dim3(64 * WR * WO), 0, s, a);
+static void ring_launch(RingArgs a, hipStream_t s) {
+  constexpr int OT = ring_outputs(NX, NW);
+  a.out_tiles = (a.out32 + 8 * OT - 1) / (8 * OT);
+  if (a.cols < 64) {
+    hipLaunchKernelGGL((ring_rows_kernel<NX, NW, 8>), dim3(a.out32, a.row_tiles), dim3(512), 0, s, a);
+    return;
   }
+  const int parts = !a.ws ? 1 : ring_parts((size_t)a.out_tiles * a.row_tiles, a.k32 / 2);
+  if (parts == 1) a.ws = nullptr;
+  const u64 mask = a.mask;
+  if (a.ws) a.mask = ~u64(0);
+  const int blocks = a.row_tiles >= 8 ? (a.row_tiles + 7) / 8 * 8 * a.out_tiles : (a.row_tiles * a.out_tiles + 7) / 8 * 8;
+  const dim3 grid(blocks, parts);
+  if (a.x1) hipLaunchKernelGGL((ring_tile_kernel<NX, NW, OT, true>), grid, dim3(512), 0, s, a);
+  else hipLaunchKernelGGL((ring_tile_kernel<NX, NW, OT, false>), grid, dim3(512), 0, s, a);
+  a.mask = mask;
+  if (a.ws) hipLaunchKernelGGL(ring_join_kernel, dim3((a.n_out + 255) / 256, (unsigned)a.n_rows), dim3(256), 0, s, a, parts);
 }
 // digits of x and of the weights that kernels exist for (x: what the ring needs, rounded up; weights: 1..4 or all)
 static int ring_digits_x(int bw) { return bw <= 32 ? 4 : bw <= 40 ? 5 : bw <= 48 ? 6 : 8; }
@@ -446,8 +538,8 @@ extern "C" int mmh_ring_weights_create(const void *d_w, int elem_bytes, size_t n
   MMH_REQUIRE(h, MMH_ERR_MEMORY);
   h->groups = n_groups, h->rows = rows, h->cols = cols, h->bw = ring_bw;
   h->nx = ring_digits_x(ring_bw);
-  h->k64 = (cols + 63) / 64, h->out16 = (rows + 15) / 16;
-  const size_t frags = n_groups * h->out16 * h->k64;
+  h->k32 = (cols + 63) / 64 * 2, h->out32 = (rows + 31) / 32;
+  const size_t frags = n_groups * h->out32 * h->k32;
   int need = 0, *d_need = nullptr;
   auto fail = [&](int code, const char *what, hipError_t e) {
     (void)hipGetLastError();
@@ -459,7 +551,7 @@ extern "C" int mmh_ring_weights_create(const void *d_w, int elem_bytes, size_t n
   };
   hipError_t e = hipGetDevice(&h->device);
   if (e != hipSuccess) return fail(MMH_ERR_INTERNAL, "hipGetDevice", e);
-  if (frags / n_groups / h->out16 != h->k64 || frags >= (size_t(1) << 31) || n_groups * rows * cols / rows / cols != n_groups)
+  if (frags / n_groups / h->out32 != h->k32 || frags >= (size_t(1) << 31) || n_groups * rows * cols / rows / cols != n_groups)
     return fail(MMH_ERR_OUT_BOUND, "too many weights", hipSuccess);
   e = hipMalloc((void **)&d_need, sizeof(int));
   if (e != hipSuccess) return fail(MMH_ERR_MEMORY, "hipMalloc", e);
@@ -505,16 +597,34 @@ extern "C" int mmh_ring_weights_info(const mmh_ring_weights *w, size_t *n_groups
   if (digits) *digits = w->nw;
   return MMH_OK;
 }
+namespace mmh {
+// row tiles of 32 rows that the groups can have: each nonempty group has at most one that is not full
+static size_t ring_row_tiles(const mmh_ring_weights *w, size_t n_rows, bool offsets) {
+  return offsets ? n_rows / 32 + std::min(w->groups, n_rows) : (n_rows + 31) / 32;
+}
+static size_t ring_ws_words(const mmh_ring_weights *w, size_t n_rows, size_t row_tiles) {
+  const int ot = 8 * ring_outputs(w->nx, w->nw);
+  const int parts = w->cols < 64 ? 1 : ring_parts(row_tiles * ((w->out32 + ot - 1) / ot), w->k32 / 2);
+  return parts > 1 ? parts * n_rows * w->rows : 0;
+}
+}  // namespace mmh
+extern "C" int mmh_ring_matmul_workspace(const mmh_ring_weights *w, size_t n_rows, size_t *words) {
+  MMH_REQUIRE(w && words, MMH_ERR_NULL_POINTER);
+  // with offsets or without: the larger of the two
+  *words = std::max(ring_ws_words(w, n_rows, ring_row_tiles(w, n_rows, true)), ring_ws_words(w, n_rows, ring_row_tiles(w, n_rows, false)));
+  return MMH_OK;
+}
 extern "C" int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, size_t ldx, const uint64_t *d_x1, size_t ldx1,
                                size_t n_tokens, const int64_t *d_rows, const int64_t *d_offsets, size_t n_rows,
-                               const uint64_t *d_add, size_t ldadd, uint64_t *d_out, size_t ldo, void *stream) {
+                               const uint64_t *d_add, size_t ldadd, uint64_t *d_out, size_t ldo, int zero_rest, uint64_t *d_ws, size_t ws_words,
+                               void *stream) {
   MMH_REQUIRE(w, MMH_ERR_NULL_POINTER);
   DeviceScope scope(w->device);
   if (scope.rc) MMH_FAIL(scope.rc, "cannot make the weights' device current");
   if (n_rows == 0) return MMH_OK;
-  MMH_REQUIRE(d_out && (d_x || n_tokens == 0), MMH_ERR_NULL_POINTER);
+  MMH_REQUIRE(d_out && d_x, MMH_ERR_NULL_POINTER);
   MMH_REQUIRE(d_offsets || w->groups == 1, MMH_ERR_NULL_POINTER);
-  MMH_REQUIRE(d_rows || n_rows <= n_tokens, MMH_ERR_DIM_MISMATCH);
+  MMH_REQUIRE(n_tokens >= 1 && (d_rows || n_rows <= n_tokens), MMH_ERR_DIM_MISMATCH);
   MMH_REQUIRE(ldx >= w->cols && (!d_x1 || ldx1 >= w->cols) && ldo >= w->rows, MMH_ERR_DIM_MISMATCH);
   MMH_REQUIRE(!d_add || ldadd == 0 || ldadd >= w->rows, MMH_ERR_DIM_MISMATCH);
   // row tiles are the second dimension of the grid, which the hardware counts in 16 bits
@@ -522,11 +632,11 @@ extern "C" int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, s
   RingArgs a;
   a.w = w->d, a.x = d_x, a.x1 = d_x1, a.add = d_add, a.rows = d_rows, a.offsets = d_offsets, a.out = d_out;
   a.ldx = ldx, a.ldx1 = ldx1, a.ldadd = ldadd, a.ldo = ldo, a.n_tokens = n_tokens, a.n_rows = n_rows;
-  a.groups = (int)w->groups, a.cols = (int)w->cols, a.n_out = (int)w->rows, a.k64 = (int)w->k64, a.out16 = (int)w->out16;
+  a.ws = nullptr, a.out_tiles = 0, a.zero_rest = zero_rest;
+  a.groups = (int)w->groups, a.cols = (int)w->cols, a.n_out = (int)w->rows, a.k32 = (int)w->k32, a.out32 = (int)w->out32;
   a.mask = w->bw >= 64 ? ~u64(0) : (u64(1) << w->bw) - 1;
-  auto aligned = [](const void *p, size_t ld) { return ((uintptr_t)p & 15) == 0 && (ld & 1) == 0; };
-  a.vec_x = aligned(d_x, ldx) && (!d_x1 || aligned(d_x1, ldx1));
-  a.vec_out = aligned(d_out, ldo);
+  a.row_tiles = (int)ring_row_tiles(w, n_rows, d_offsets != nullptr);
+  a.ws = d_ws && ws_words >= ring_ws_words(w, n_rows, a.row_tiles) ? d_ws : nullptr;
   hipStream_t s = (hipStream_t)stream;
   bool ok = false;
   if (w->nx == 4) ok = ring_dispatch_w<4>(w->nw, a, s);

@@ -172,7 +172,8 @@ SIGNATURES = {
     "mmh_ring_weights_create": [_vp, _int, _sz, _sz, _sz, _int, _vp, C.POINTER(_vp)],
     "mmh_ring_weights_destroy": [_vp],
     "mmh_ring_weights_info": [_vp, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_int), C.POINTER(_int)],
-    "mmh_ring_matmul": [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp],
+    "mmh_ring_matmul": [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _int, _vp, _sz, _vp],
+    "mmh_ring_matmul_workspace": [_vp, _sz, C.POINTER(_sz)],
     "mmh_rotary": [_vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp, _sz, _int, C.c_double, _int, _int, _vp, _sz, _sz, _vp],
     "mmh_rotary_trunc_pre": [_int, _vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp, _sz, _int, C.c_double, _int, _int, _int, _int, _vp,
                              _vp, _vp],

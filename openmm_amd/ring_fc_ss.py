@@ -13,6 +13,8 @@ to which expert is public.  Same ``gemini::Code`` errors as the other layer clas
 """
 import ctypes as C
 
+import torch
+
 from . import lib as L
 
 
@@ -21,22 +23,23 @@ def _need(cond, code, what):
         raise L.MMHError(code, what)
 
 
-def _rows_of(t, what, cols=None):
-    """a 2-D int64 CUDA tensor with contiguous rows -> its row stride in words"""
-    import torch
-    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int64 and t.dim() == 2, 7,
-          f"{what}: expected a 2-D int64 CUDA tensor")
-    _need(cols is None or t.shape[1] == cols, 3, f"{what}: {t.shape[1]} columns instead of {cols}")
-    _need(t.shape[1] <= 1 or t.numel() == 0 or t.stride(1) == 1, 7, f"{what}: rows must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _rows_of(t, what, cols, dev):
+    """a 2-D int64 tensor on CUDA device ``dev`` with contiguous rows of ``cols`` words -> its row stride in words"""
+    if t.dtype is not torch.int64 or t.dim() != 2 or t.get_device() != dev:
+        raise L.MMHError(7, f"{what}: expected a 2-D int64 tensor on the weights' device")
+    n, c = t.shape
+    step, one = t.stride()
+    if c != cols:
+        raise L.MMHError(3, f"{what}: {c} columns instead of {cols}")
+    if one != 1 and c > 1 and n:
+        raise L.MMHError(7, f"{what}: rows must be contiguous")
+    return step if n > 1 else c
 
 
-def _index(t, what, device):
-    import torch
-    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int64 and t.dim() == 1 and t.is_contiguous(), 7,
-          f"{what}: expected a contiguous 1-D int64 tensor")
-    _need(t.device == device, 7, f"{what}: on another device than the weights")
-    return t
+def _index(t, what, dev):
+    if t.dtype is not torch.int64 or t.dim() != 1 or t.get_device() != dev or not t.is_contiguous():
+        raise L.MMHError(7, f"{what}: expected a contiguous 1-D int64 tensor on the weights' device")
+    return t.shape[0]
 
 
 class RingWeights:
@@ -44,14 +47,14 @@ class RingWeights:
     integers int8 / int16 / int32 / int64 on the GPU; congruent modulo 2^ring_bw is the same weight."""
 
     def __init__(self, w, ring_bw):
-        import torch
         self.handle = L._vp()
         self.lib = L.load_library()
         _need(isinstance(w, torch.Tensor) and w.is_cuda and w.dtype in (torch.int8, torch.int16, torch.int32, torch.int64), 7,
               "encodeWeights: expected an int8, int16, int32 or int64 CUDA tensor")
         _need(w.dim() in (2, 3), 3, "encodeWeights: weight shape")
         w = w.contiguous()
-        self.device = w.device
+        self.device = w.get_device()
+        self._words = {}
         g, rows, cols = w.shape if w.dim() == 3 else (1, *w.shape)
         with torch.cuda.device(w.device):
             L.check(self.lib.mmh_ring_weights_create(L.dptr(w), w.element_size(), g, rows, cols, ring_bw, L._stream_ptr(),
@@ -59,6 +62,17 @@ class RingWeights:
         d = L._int()
         L.check(self.lib.mmh_ring_weights_info(self.handle, None, None, None, None, C.byref(d)))
         self.groups, self.rows, self.cols, self.ring_bw, self.digits = g, rows, cols, ring_bw, d.value
+
+    def workspace(self, n):
+        """scratch words of a call of n rows"""
+        words = self._words.get(n)
+        if words is None:
+            c = L._sz()
+            L.check(self.lib.mmh_ring_matmul_workspace(self.handle, n, C.byref(c)))
+            if len(self._words) >= 256:
+                self._words.clear()
+            words = self._words[n] = c.value
+        return words
 
     def close(self):
         if self.handle:
@@ -91,35 +105,47 @@ class RingFCSS:
         """out[r] = add[r] + W_g (x[t] + share1[t]) mod 2^l for offsets[g] <= r < offsets[g + 1], t = rows[r].
 
         x, share1 [tokens, cols]; rows int64 [n] (None: row r reads token r); offsets int64 [groups + 1] on the device (None
-        with one group); add [n, w.rows] or [w.rows]; out [n, w.rows] (a new tensor of zeros behind the last group when
-        None).  2-D operands may have any row stride.  add may be out."""
-        import torch
-        _need(self.ring_bw is not None, 1, "matMul: setUp first")
-        _need(isinstance(weights, RingWeights) and bool(weights.handle) and weights.ring_bw == self.ring_bw, 7, "matMul: weights")
-        ldx = _rows_of(x, "matMul: x", weights.cols)
-        _need(x.device == weights.device, 7, "matMul: x on another device than the weights")
-        tokens, ldx1 = x.shape[0], 0
+        with one group); add [n, w.rows] or [w.rows]; out [n, w.rows] (a new tensor with zeros in rows of no group
+        when None).  2-D operands may have any row stride.  add may be out."""
+        if self.ring_bw is None:
+            raise L.MMHError(1, "matMul: setUp first")
+        if not isinstance(weights, RingWeights) or not weights.handle or weights.ring_bw != self.ring_bw:
+            raise L.MMHError(7, "matMul: weights")
+        dev, cols, wide = weights.device, weights.cols, weights.rows
+        ldx = _rows_of(x, "matMul: x", cols, dev)
+        n = tokens = x.shape[0]
+        px1 = ldx1 = prows = poff = padd = ldadd = pws = 0
         if share1 is not None:
-            ldx1 = _rows_of(share1, "matMul: share1", weights.cols)
-            _need(share1.shape[0] == tokens and share1.device == x.device, 3, "matMul: #shares")
-        n = tokens if rows is None else _index(rows, "matMul: rows", x.device).numel()
-        if offsets is None:
-            _need(weights.groups == 1, 2, "matMul: offsets")
+            ldx1, px1 = _rows_of(share1, "matMul: share1", cols, dev), share1.data_ptr()
+            _need(share1.shape[0] == tokens, 3, "matMul: #shares")
+        if rows is not None:
+            n, prows = _index(rows, "matMul: rows", dev), rows.data_ptr()
+        if offsets is not None:
+            _need(_index(offsets, "matMul: offsets", dev) == weights.groups + 1, 3, "matMul: offsets")
+            poff = offsets.data_ptr()
         else:
-            _need(_index(offsets, "matMul: offsets", x.device).numel() == weights.groups + 1, 3, "matMul: offsets")
-        ldadd = 0
+            _need(weights.groups == 1, 2, "matMul: offsets")
         if add is not None:
-            ldadd = _rows_of(add if add.dim() == 2 else add[None], "matMul: add", weights.rows)
-            ldadd = ldadd if add.dim() == 2 else 0
-            _need((add.dim() == 1 or add.shape[0] == n) and add.device == x.device, 3, "matMul: add")
-        if out is None:
-            # with offsets, rows behind the last group are not written
-            new = torch.empty if offsets is None else torch.zeros
-            out = new((n, weights.rows), dtype=torch.int64, device=x.device)
-        ldo = _rows_of(out, "matMul: out", weights.rows)
-        _need(out.shape[0] == n and out.device == x.device, 3, "matMul: out")
-        ptr = lambda t: L._vp(0 if t is None else t.data_ptr())
-        s = L._vp(torch.cuda.current_stream(x.device).cuda_stream)
-        L.check(weights.lib.mmh_ring_matmul(weights.handle, ptr(x), ldx, ptr(share1), ldx1, tokens, ptr(rows), ptr(offsets), n,
-                                            ptr(add), ldadd, ptr(out), ldo, s))
+            padd = add.data_ptr()
+            if add.dim() == 1:
+                _rows_of(add[None], "matMul: add", wide, dev)
+            else:
+                ldadd = _rows_of(add, "matMul: add", wide, dev)
+                _need(add.shape[0] == n, 3, "matMul: add")
+        new = out is None
+        if new:
+            out, ldo = torch.empty((n, wide), dtype=torch.int64, device=x.device), wide
+        else:
+            ldo = _rows_of(out, "matMul: out", wide, dev)
+            _need(out.shape[0] == n, 3, "matMul: out")
+        if n == 0:
+            return out
+        words = weights.workspace(n)
+        if words:
+            ws = torch.empty(words, dtype=torch.int64, device=x.device)
+            pws = ws.data_ptr()
+        rc = weights.lib.mmh_ring_matmul(weights.handle, x.data_ptr(), ldx, px1, ldx1, tokens, prows, poff, n, padd, ldadd,
+                                         out.data_ptr(), ldo, new, pws, words, torch._C._cuda_getCurrentRawStream(dev))
+        if rc:
+            L.check(rc)
         return out

@@ -7,6 +7,8 @@ integers computed with decimal arithmetic and do not depend on a machine's mathe
 """
 from decimal import Decimal, localcontext
 
+import torch
+
 from . import lib as L
 from .ring_fc_ss import _need
 from .truncation import ALICE, BOB
@@ -52,7 +54,6 @@ class Rotary:
     2^frac_bits.  Pairs are (i, i + len(phases)), or (2i, 2i + 1) when interleaved."""
 
     def __init__(self, phases, head_dim, frac_bits, ring_bw, interleaved=False, amplitude=1.0, device="cuda:0"):
-        import torch
         self.lib = L.load_library()
         if not isinstance(phases, torch.Tensor):
             phases = torch.tensor([p - (1 << 64) if p >= 1 << 63 else p for p in phases], dtype=torch.int64, device=device)
@@ -63,45 +64,57 @@ class Rotary:
         self.phases, self.head_dim, self.frac_bits, self.ring_bw = phases, head_dim, frac_bits, ring_bw
         self.interleaved, self.amplitude = bool(interleaved), float(amplitude)
 
-    def _check(self, x, positions):
-        import torch
-        _need(isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.int64 and x.dim() == 3, 7,
-              "Rotary: expected a 3-D int64 CUDA tensor [tokens, heads, head_dim]")
-        _need(x.shape[2] == self.head_dim, 3, "Rotary: head_dim")
-        _need(x.numel() == 0 or x.shape[2] == 1 or x.stride(2) == 1, 7, "Rotary: the words of a head must be contiguous")
-        _need(isinstance(positions, torch.Tensor) and positions.dtype == torch.int64 and positions.dim() == 1 and
-              positions.is_contiguous(), 7, "Rotary: expected contiguous int64 positions")
-        _need(positions.numel() == x.shape[0], 3, "Rotary: #positions")
-        _need(positions.device == x.device and self.phases.device == x.device, 7, "Rotary: operands on different devices")
+        self._dev = phases.get_device()
+        self._pairs = (phases.data_ptr(), 2 * phases.numel(), self.interleaved, self.amplitude, self.frac_bits, self.ring_bw)
+
+    def _check(self, x):
+        if x.dtype is not torch.int64 or x.dim() != 3 or x.get_device() != self._dev:
+            raise L.MMHError(7, "Rotary: expected a 3-D int64 tensor [tokens, heads, head_dim] on the phases' device")
+        if x.shape[2] != self.head_dim:
+            raise L.MMHError(3, "Rotary: head_dim")
+        if x.stride(2) != 1 and self.head_dim != 1 and x.numel():
+            raise L.MMHError(7, "Rotary: the words of a head must be contiguous")
 
     def _args(self, x, positions):
-        return (L._vp(x.data_ptr()), x.stride(0), x.stride(1), x.shape[0], x.shape[1], self.head_dim,
-                L._vp(positions.data_ptr()), L._vp(self.phases.data_ptr()), 2 * self.phases.numel(), int(self.interleaved),
-                self.amplitude, self.frac_bits, self.ring_bw)
+        self._check(x)
+        if positions.dtype is not torch.int64 or positions.dim() != 1 or positions.get_device() != self._dev or \
+                not positions.is_contiguous():
+            raise L.MMHError(7, "Rotary: expected contiguous int64 positions on the phases' device")
+        tokens, heads, dim = x.shape
+        if positions.shape[0] != tokens:
+            raise L.MMHError(3, "Rotary: #positions")
+        st, sh, _ = x.stride()
+        return (x.data_ptr(), st, sh, tokens, heads, dim, positions.data_ptr(), *self._pairs)
+
+    def _call(self, fn, *args):
+        stream = torch._C._cuda_getCurrentRawStream(self._dev)
+        if torch.cuda.current_device() == self._dev:
+            rc = fn(*args, stream)
+        else:
+            with torch.cuda.device(self._dev):
+                rc = fn(*args, stream)
+        if rc:
+            L.check(rc)
 
     def rotate(self, x, positions, out=None):
         """the turned share, scaled by 2^frac_bits; ``out`` may be x (same strides), or another tensor of the shape"""
-        import torch
-        self._check(x, positions)
+        args = self._args(x, positions)
         if out is None:
             out = torch.empty(x.shape, dtype=torch.int64, device=x.device)
         else:
-            self._check(out, positions)
+            self._check(out)
             _need(out.shape == x.shape, 3, "Rotary: out")
-        with torch.cuda.device(x.device):
-            L.check(self.lib.mmh_rotary(*self._args(x, positions), L._vp(out.data_ptr()), out.stride(0), out.stride(1),
-                                        L._stream_ptr()))
+        st, sh, _ = out.stride()
+        self._call(self.lib.mmh_rotary, *args, out.data_ptr(), st, sh)
         return out
 
     def truncate_pre(self, party, x, positions, signed_arithmetic=True, apply_msb0_heuristic=True):
         """the turned share as the truncation's wrap protocol takes it, and the operand of its comparison (None with the
         heuristic, which does not compare)"""
-        import torch
         _need(party in (ALICE, BOB), 7, "Rotary: party")
-        self._check(x, positions)
+        args = self._args(x, positions)
         adj = torch.empty(x.shape, dtype=torch.int64, device=x.device)
         cmp = None if apply_msb0_heuristic else torch.empty_like(adj)
-        with torch.cuda.device(x.device):
-            L.check(self.lib.mmh_rotary_trunc_pre(party, *self._args(x, positions), int(signed_arithmetic),
-                                                  int(apply_msb0_heuristic), L.dptr(adj), L.dptr(cmp), L._stream_ptr()))
+        self._call(self.lib.mmh_rotary_trunc_pre, party, *args, bool(signed_arithmetic), bool(apply_msb0_heuristic),
+                   adj.data_ptr(), 0 if cmp is None else cmp.data_ptr())
         return adj, cmp

@@ -244,10 +244,10 @@ def test_refusals(mm):
     px, po, y = vp(x.data_ptr()), vp(off.data_ptr()), z(4, 8)
     py = vp(y.data_ptr())
     raw = lambda x=px, ldx=12, x1=None, ldx1=0, t=4, rows=None, off=po, n=4, add=None, lda=0, out=py, ldo=8: \
-        lib.mmh_ring_matmul(rw.handle, x, ldx, x1, ldx1, t, rows, off, n, add, lda, out, ldo, None)
+        lib.mmh_ring_matmul(rw.handle, x, ldx, x1, ldx1, t, rows, off, n, add, lda, out, ldo, 0, None, 0, None)
     assert raw() == 0 and raw(n=0, x=None, out=None) == 0
     assert raw(x=None) == 2 and raw(out=None) == 2 and raw(off=None) == 2
-    assert raw(t=3) == 3 and raw(ldx=11) == 3 and raw(x1=px, ldx1=11) == 3 and raw(ldo=7) == 3 and raw(add=py, lda=7) == 3
+    assert raw(t=0, rows=po) == 3 and raw(t=3) == 3 and raw(ldx=11) == 3 and raw(x1=px, ldx1=11) == 3 and raw(ldo=7) == 3 and raw(add=py, lda=7) == 3
     assert raw(n=(1 << 19) + 1, t=1 << 20) == 6
     rw.close()
     with pytest.raises(MMHError):

@@ -25,7 +25,8 @@ def test_ring_product_refusals_without_gpu():
     assert not h and b"mmh_ring_weights_create" in lib.mmh_last_error()
     assert lib.mmh_ring_weights_info(None, None, None, None, None, None) == 2
     assert lib.mmh_ring_weights_destroy(None) == 0
-    assert lib.mmh_ring_matmul(None, P, 4, None, 0, 1, None, None, 1, None, 0, P, 4, None) == 2
+    assert lib.mmh_ring_matmul(None, P, 4, None, 0, 1, None, None, 1, None, 0, P, 4, 0, None, 0, None) == 2
+    assert lib.mmh_ring_matmul_workspace(None, 1, C.byref(C.c_size_t())) == 2
 
 
 def test_rotary_refusals_without_gpu():
