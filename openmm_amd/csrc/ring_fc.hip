@@ -187,13 +187,16 @@ __device__ __forceinline__ void ring_store_digits(uint4 *frag, int row, int k16,
   for (int d = 0; d < NX; ++d) reinterpret_cast<u32 *>(&frag[d * 64 + k16 * 32 + row])[sub] = dig[d];
 }
 __device__ __forceinline__ v4i as_v4i(const uint4 &t) { return v4i{(int)t.x, (int)t.y, (int)t.z, (int)t.w}; }
-// the 64-bit value of element e of a 32 x 32 tile from its digit sums
-template <int NX>
-__device__ __forceinline__ u64 ring_value(const v16i (&acc)[NX], int e) {
-  u64 v = 0;
+// sum_s 256^s acc_s mod 2^64: what lies at 2^32 and above in 32-bit arithmetic
+template <int NX, typename T>
+__device__ __forceinline__ u64 ring_value(const T (&acc)[NX], int e) {
+  u64 v = (u64)(long long)acc[0][e];
 #pragma unroll
-  for (int s = NX - 1; s >= 0; --s) v = (v << 8) + (u64)(long long)acc[s][e];
-  return v;
+  for (int s = 1; s < NX && s < 4; ++s) v += (u64)((long long)acc[s][e] * (1 << 8 * s));
+  u32 h = hi32(v);
+#pragma unroll
+  for (int s = 4; s < NX; ++s) h += (u32)acc[s][e] << (8 * (s - 4));
+  return make64(lo32(v), h);
 }
 
 // first column of fragment c: steps of two fragments, the last of which ends with the last column (weights of columns that the
@@ -261,6 +264,103 @@ __global__ __launch_bounds__(64 * WK, 2) void ring_rows_kernel(RingArgs a) {
   }
 }
 
+// Up to 8 rows: a workgroup computes them for 16 outputs, its 16 waves split k in steps of 64 columns and join their 64-bit sums
+// through LDS.  Bound by latency: everything a wave needs of its first steps is asked for at once (kAhead steps), and it cuts
+// its own digits into LDS of its own, so the loop has no barrier.  16 x 16 products (v_mfma_i32_16x16x64_i8), of whose rows 8
+// stay zero: their rate does not matter here, their few registers do.  Needs 64 columns or more.
+template <int NX, int NW, bool TWO>
+__global__ __launch_bounds__(1024) void ring_few_kernel(RingArgs a) {
+  constexpr int W = 16, kAhead = NW <= 2 && !TWO ? 2 : 1;
+  __shared__ uint4 lds[W][NX * 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int ot = (int)blockIdx.x;   // 16 outputs
+  if (blockIdx.y == 0) ring_zero_rest(a, ot * 16, ot * 16 + 16);
+  int g;
+  size_t lo, hi;
+  if (!ring_find_tile<8>(a, blockIdx.y, g, lo, hi)) return;
+  // a lane cuts four words of rows lane % 4 and, with more than four rows, lane % 4 + 4
+  const int r = lane & 3, k4 = lane >> 2;
+  const bool eight = hi - lo > 4;
+  const u64 *px[2], *px1[2];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const size_t row = lo + 4 * b + r;
+    const long long t = row < hi ? ring_token(a, row) : -1;
+    const size_t token = t < 0 ? 0 : (size_t)t;   // any row will do: its sums are not used
+    px[b] = a.x + token * a.ldx + k4 * 4, px1[b] = TWO ? a.x1 + token * a.ldx1 + k4 * 4 : nullptr;
+  }
+  // 16 outputs x 64 columns of a step's two fragments: lane (quarter, output) reads 16 columns
+  const int8_t *pw = a.w + ((size_t)g * a.out32 + (ot >> 1)) * a.k32 * (NW * 1024) + (lane >> 5) * (NW * 1024) +
+                     (lane >> 4 & 1) * 512 + ((ot & 1) * 16 + (lane & 15)) * 16;
+  const int last = a.k32 / 2 - 1;
+  struct Step {
+    v4i w[NW];
+    u64 x[2][4], x1[TWO ? 2 : 1][4];
+  } s[kAhead];
+  auto load = [&](Step &v, int c) {
+    c = c < last ? c : last;
+    const int k = c * 64 < a.cols - 64 ? c * 64 : a.cols - 64;   // the last step ends with the last column
+#pragma unroll
+    for (int j = 0; j < NW; ++j) v.w[j] = *reinterpret_cast<const v4i *>(pw + ((size_t)2 * c * NW + j) * 1024);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      if (b == 0 || eight) {
+        ring_load4(px[b] + k, v.x[b]);
+        if constexpr (TWO) ring_load4(px1[b] + k, v.x1[b]);
+      }
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load(s[i], wave + i * W);
+#pragma unroll
+  for (int i = 0; i < NX; ++i) lds[wave][i * 64 + lane] = make_uint4(0, 0, 0, 0);
+  v4i acc[NX];
+#pragma unroll
+  for (int i = 0; i < NX; ++i) acc[i] = v4i{0, 0, 0, 0};
+  auto step = [&](Step &v, int c) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      if (b == 0 || eight) {
+        u64 t[4];
+        u32 dig[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = TWO ? v.x[b][e] + v.x1[TWO ? b : 0][e] : v.x[b][e];
+        ring_digits4<NX>(t, dig);
+#pragma unroll
+        for (int d = 0; d < NX; ++d) reinterpret_cast<u32 *>(&lds[wave][d * 64 + (k4 >> 2) * 16 + 4 * b + r])[k4 & 3] = dig[d];
+      }
+    v4i w[NW];
+#pragma unroll
+    for (int j = 0; j < NW; ++j) w[j] = v.w[j];
+    if (c + kAhead * W <= last) load(v, c + kAhead * W);
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      const v4i x = as_v4i(lds[wave][i * 64 + lane]);
+#pragma unroll
+      for (int j = 0; j < NW; ++j)
+        if (i + j < NX) acc[i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x, acc[i + j], 0, 0, 0);
+    }
+  };
+  for (int c = wave; c <= last; c += kAhead * W)
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (c + i * W <= last) step(s[i], c + i * W);
+  // element e of a lane: row lane % 16, output 4 * (lane / 16) + e
+  __syncthreads();
+  u64 *part = reinterpret_cast<u64 *>(&lds[0][0]);   // [wave][row][output]
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if ((lane & 15) < 8) part[(wave * 8 + (lane & 15)) * 16 + (lane >> 4) * 4 + e] = ring_value<NX>(acc, e);
+  }
+  __syncthreads();
+  const int i = (int)threadIdx.x, row = i >> 4, n = ot * 16 + (i & 15);
+  if (i >= 128 || lo + row >= hi || n >= a.n_out) return;
+  u64 v = a.add ? a.add[(lo + row) * a.ldadd + n] : 0;
+  if (ring_token(a, lo + row) >= 0)
+#pragma unroll
+    for (int k = 0; k < W; ++k) v += part[(k * 8 + row) * 16 + (i & 15)];
+  a.out[(lo + row) * a.ldo + n] = v & a.mask;
+}
+
 // Large products: a workgroup of 8 waves computes 32 rows x 256*OT outputs in steps of 64 columns.  The rows' digits are cut
 // once per workgroup into LDS (three buffers, one barrier per step); the weights' fragments come straight from L2 in the order
 // they were laid out in.  Words and weights are loaded into registers two steps before they are used; nothing in the loop
@@ -282,20 +382,23 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
   const size_t token = my_token < 0 ? 0 : (size_t)my_token;   // any row will do: its sums are not used
   const int in_step = (wave >> 1) * 16 + sub * 4;
   const u64 *px = a.x + token * a.ldx + in_step, *px1 = TWO ? a.x1 + token * a.ldx1 + in_step : nullptr;
-  u64 xv[2][4], xu[2][4];
+  struct Words {
+    u64 x[4], x1[TWO ? 4 : 1];
+  };
+  Words words[2];
   const int last = a.k32 / 2 - 1;
-  auto load_x = [&](int p, int c) {
+  auto load_x = [&](Words &v, int c) {
     c = c < last ? c : last;
     const int k = c * 64 < a.cols - 64 ? c * 64 : a.cols - 64;   // the last step ends with the last column
-    ring_load4(px + k, xv[p]);
-    if (TWO) ring_load4(px1 + k, xu[p]);
+    ring_load4(px + k, v.x);
+    if constexpr (TWO) ring_load4(px1 + k, v.x1);
   };
   // half 0: digits 0 .. 3, half 1: the others
-  auto store_x = [&](int p, int buf, int half) {
+  auto store_x = [&](const Words &v, int buf, int half) {
     u32 d[4];
     u64 t[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) t[e] = (TWO ? xv[p][e] + xu[p][e] : xv[p][e]) + kDigitBias;
+    for (int e = 0; e < 4; ++e) t[e] = (TWO ? v.x[e] + v.x1[TWO ? e : 0] : v.x[e]) + kDigitBias;
     if (half == 0) transpose4(lo32(t[0]), lo32(t[1]), lo32(t[2]), lo32(t[3]), d);
     else transpose4(hi32(t[0]), hi32(t[1]), hi32(t[2]), hi32(t[3]), d);
     uint4 *frag = xs[buf] + (wave >> 2) * (NX * 64) + (wave >> 1 & 1) * 32 + (wave & 1) * 16 + r;
@@ -341,10 +444,10 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
         for (int j = 0; j < NW; ++j)
           if (i + j < NX)
             acc[o][i + j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[p][h][o][j], f[t % (D + 1)], acc[o][i + j], 0, 0, 0);
-      if (t == kCut) store_x(p, wr, 0);
-      if (NX > 4 && t == kCut + 2) store_x(p, wr, 1);
+      if (t == kCut) store_x(words[p], wr, 0);
+      if (NX > 4 && t == kCut + 2) store_x(words[p], wr, 1);
       if (t == NX - 1) {
-        load_x(p, c + 4);
+        load_x(words[p], c + 4);
         load_w(p, 0, c + 2);
         barrier();
       }
@@ -360,20 +463,21 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
   const int end = (int)((long long)(last + 1) * (blockIdx.y + 1) / gridDim.y);
   for (int c0 = first; c0 < end; c0 += kFlush) {
     const int c1 = c0 + kFlush < end ? c0 + kFlush : end;
+    Words one, two;
+    load_x(one, c0);
+    load_x(two, c0 + 1);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) load_w(p, 0, c0 + p), load_w(p, 1, c0 + p);
+    load_x(words[0], c0 + 2);
+    load_x(words[1], c0 + 3);
+#pragma unroll
+    for (int half = 0; half < (NX > 4 ? 2 : 1); ++half) store_x(one, rd, half), store_x(two, nx, half);
 #pragma unroll
     for (int o = 0; o < OT; ++o)
 #pragma unroll
       for (int s = 0; s < NX; ++s)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[o][s][e] = 0;
-    load_x(0, c0);
-    load_x(1, c0 + 1);
-#pragma unroll
-    for (int p = 0; p < 2; ++p) load_w(p, 0, c0 + p), load_w(p, 1, c0 + p);
-#pragma unroll
-    for (int half = 0; half < (NX > 4 ? 2 : 1); ++half) store_x(0, rd, half), store_x(1, nx, half);
-    load_x(0, c0 + 2);
-    load_x(1, c0 + 3);
     barrier();
 #pragma unroll
     for (int t = 0; t < D; ++t) f[t] = as_v4i(xs[rd][t * 64 + lane]);
@@ -477,22 +581,41 @@ static void ring_launch_layout(const void *w, const mmh_ring_weights *h, hipStre
                      h->rows, h->cols, h->bw, h->out32, h->k32, h->nw, units, h->d);
 }
 
-// parts of k for `tiles` workgroups of the tile kernel: fill the chip's 256 compute units, four steps or more each
-static int ring_parts(size_t tiles, size_t steps) {
-  return (int)std::max<size_t>(1, std::min(std::min<size_t>(256 / std::max<size_t>(tiles, 1), steps / 4), size_t(16)));
+// Parts of k for `tiles` workgroups of the tile kernel on the chip's 256 compute units, by a model of its time (us): rounds of
+// workgroups, each with its steps and a start and end of its own, and the launch that adds up the parts, 16 bytes of traffic
+// per part and output.  A step of 30 products takes 2 us with all units busy, a few products no less than 1.
+static int ring_parts(size_t tiles, size_t steps, int products, size_t outputs) {
+  const double step = std::max(1.0, products * (2.0 / 30));
+  int best = 1;
+  double least = 0;
+  for (int p = 1; p <= 16 && (size_t)p * 2 <= std::max<size_t>(steps, 2); ++p) {
+    const double rounds = (double)((tiles * p + 255) / 256);
+    const double t = rounds * ((double)((steps + p - 1) / p) * step + 5) + (p > 1 ? 5 + p * (double)outputs * 16 / 4.5e6 : 0);
+    if (p == 1 || t < 0.95 * least) best = p, least = t;
+  }
+  return best;
 }
+// up to 8 rows in all go to ring_few_kernel, whose waves must not sum more columns than fit 32 bits
+static bool ring_few(size_t n_rows, size_t cols, int nw) { return n_rows <= 8 && cols >= 64 && (cols / 64 / 16 + 1) * 64 * nw <= 131071; }
+static constexpr int ring_products(int nx, int nw) { return 2 * (nx * nw - nw * (nw - 1) / 2); }   // of a 64-column step
 // 32-output tiles a wave computes: the accumulators of one take 16 nx registers; two while they fit, for fewer digit reads
 static constexpr int ring_outputs(int nx, int nw) { return nx * 32 + nw * 32 <= 160 ? 2 : 1; }
 
 template <int NX, int NW>
 static void ring_launch(RingArgs a, hipStream_t s) {
   constexpr int OT = ring_outputs(NX, NW);
+  if (ring_few(a.n_rows, a.cols, NW)) {
+    const dim3 grid((a.n_out + 15) / 16, a.offsets ? std::min<unsigned>(a.groups, a.n_rows) : 1);
+    if (a.x1) hipLaunchKernelGGL((ring_few_kernel<NX, NW, true>), grid, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((ring_few_kernel<NX, NW, false>), grid, dim3(1024), 0, s, a);
+    return;
+  }
   a.out_tiles = (a.out32 + 8 * OT - 1) / (8 * OT);
   if (a.cols < 64) {
     hipLaunchKernelGGL((ring_rows_kernel<NX, NW, 8>), dim3(a.out32, a.row_tiles), dim3(512), 0, s, a);
     return;
   }
-  const int parts = !a.ws ? 1 : ring_parts((size_t)a.out_tiles * a.row_tiles, a.k32 / 2);
+  const int parts = !a.ws ? 1 : ring_parts((size_t)a.out_tiles * a.row_tiles, a.k32 / 2, OT * ring_products(NX, NW), a.n_rows * a.n_out);
   if (parts == 1) a.ws = nullptr;
   const u64 mask = a.mask;
   if (a.ws) a.mask = ~u64(0);
@@ -604,7 +727,7 @@ static size_t ring_row_tiles(const mmh_ring_weights *w, size_t n_rows, bool offs
 }
 static size_t ring_ws_words(const mmh_ring_weights *w, size_t n_rows, size_t row_tiles) {
   const int ot = 8 * ring_outputs(w->nx, w->nw);
-  const int parts = w->cols < 64 ? 1 : ring_parts(row_tiles * ((w->out32 + ot - 1) / ot), w->k32 / 2);
+  const int parts = w->cols < 64 || ring_few(n_rows, w->cols, w->nw) ? 1 : ring_parts(row_tiles * ((w->out32 + ot - 1) / ot), w->k32 / 2, ot / 8 * ring_products(w->nx, w->nw), n_rows * w->rows);
   return parts > 1 ? parts * n_rows * w->rows : 0;
 }
 }  // namespace mmh
