@@ -38,62 +38,94 @@ struct RingArgs {
   int zero_rest;
 };
 
-// The rows of row tile `tile` (BM rows, tiles do not cross groups).  Every wave finds it by itself: 64 groups at a time,
-// a prefix sum of their tile counts.  Offsets are clamped to [0, n_rows], so nothing they hold leads out of bounds.
+// Row tiles of BM rows; tiles do not cross groups.  A wave looks at 64 groups at a time, a group per lane, with a prefix sum of
+// their tile counts.  Offsets are clamped to [0, n_rows], so nothing they hold leads out of bounds.
 template <int BM>
-__device__ __forceinline__ bool ring_find_tile(const RingArgs &a, u32 tile, int &g, size_t &lo, size_t &hi) {
-  if (!a.offsets) {
-    g = 0, lo = (size_t)tile * BM;
-    hi = lo + BM < a.n_rows ? lo + BM : a.n_rows;
-    return lo < a.n_rows;
-  }
-  const int lane = threadIdx.x & 63;
-  u32 before = 0;
-  for (int g0 = 0; g0 < a.groups; g0 += 64) {
-    long long s = 0, e = 0;
+struct RingGroups {
+  long long s, e;   // rows of this lane's group
+  u32 tiles, sum;   // its tiles, and those of all groups of the wave up to it
+  __device__ __forceinline__ void load(const RingArgs &a, int g0) {
+    const int lane = threadIdx.x & 63;
+    s = e = 0;
     if (g0 + lane < a.groups) {
       const long long n = (long long)a.n_rows;
       s = a.offsets[g0 + lane], e = a.offsets[g0 + lane + 1];
       s = s < 0 ? 0 : s > n ? n : s;
       e = e < s ? s : e > n ? n : e;
     }
-    const u32 tiles = (u32)((e - s + BM - 1) / BM);
-    u32 sum = tiles;
+    tiles = (u32)((e - s + BM - 1) / BM);
+    sum = tiles;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const u32 t = __shfl_up(sum, d);
       if (lane >= d) sum += t;
     }
-    const unsigned long long past = __ballot(before + sum > tile);
+  }
+  __device__ __forceinline__ u32 total() const { return __builtin_amdgcn_readlane(sum, 63); }
+};
+struct RingTile {
+  int g, ot;
+  size_t lo, hi;
+};
+// row tile `tile`; `first` holds groups 0 .. 63
+template <int BM>
+__device__ __forceinline__ bool ring_find_tile(const RingArgs &a, const RingGroups<BM> &first, u32 tile, RingTile &t) {
+  if (!a.offsets) {
+    t.g = 0, t.lo = (size_t)tile * BM;
+    t.hi = t.lo + BM < a.n_rows ? t.lo + BM : a.n_rows;
+    return t.lo < a.n_rows;
+  }
+  RingGroups<BM> w = first;
+  u32 before = 0;
+  for (int g0 = 0;;) {
+    const unsigned long long past = __ballot(before + w.sum > tile);
     if (past) {
       const int src = __ffsll(past) - 1;
-      const u32 first = before + (u32)__shfl((int)(sum - tiles), src);
-      lo = (size_t)__shfl(s, src) + (size_t)(tile - first) * BM;
-      const size_t end = (size_t)__shfl(e, src);
-      hi = lo + BM < end ? lo + BM : end;
-      g = g0 + src;
+      const u32 at = before + __builtin_amdgcn_readlane(w.sum - w.tiles, src);
+      t.lo = make64(__builtin_amdgcn_readlane(lo32(w.s), src), __builtin_amdgcn_readlane(hi32(w.s), src)) + (u64)(tile - at) * BM;
+      const size_t end = make64(__builtin_amdgcn_readlane(lo32(w.e), src), __builtin_amdgcn_readlane(hi32(w.e), src));
+      t.hi = t.lo + BM < end ? t.lo + BM : end;
+      t.g = g0 + src;
       return true;
     }
-    before += (u32)__shfl((int)sum, 63);
+    before += w.total();
+    g0 += 64;
+    if (g0 >= a.groups) return false;
+    w.load(a, g0);
   }
-  return false;
+}
+template <int BM>
+__device__ __forceinline__ u32 ring_count_tiles(const RingArgs &a, const RingGroups<BM> &first) {
+  if (!a.offsets) return (u32)((a.n_rows + BM - 1) / BM);
+  u32 n = first.total();
+  for (int g0 = 64; g0 < a.groups; g0 += 64) {
+    RingGroups<BM> more;
+    more.load(a, g0);
+    n += more.total();
+  }
+  return n;
 }
 
-// Which tile a workgroup computes.  Workgroups go round the 8 XCDs, each with an L2 of its own, so every XCD gets a contiguous
-// piece of the order "four output tiles across, row tiles down": the workgroups that run there at one time share rows and
-// weights.
-__device__ __forceinline__ bool ring_block(const RingArgs &a, int &ot, int &rt) {
-  // with eight row tiles or more an XCD takes every eighth of them, so that tiles no group has are spread evenly
-  const bool deal = a.row_tiles >= 8;
-  const u32 rows = deal ? (a.row_tiles + 7) / 8 : a.row_tiles, total = (u32)a.out_tiles * rows, per = deal ? total : (total + 7) / 8;
-  const u32 q = (deal ? 0 : (blockIdx.x & 7) * per) + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= per || q >= total) return false;
-  const u32 panel = q / (4 * rows), rest = q - panel * 4 * rows;
-  const u32 wide = (u32)a.out_tiles - panel * 4 < 4 ? (u32)a.out_tiles - panel * 4 : 4;
-  rt = (int)(rest / wide), ot = (int)(panel * 4 + rest % wide);
-  if (deal) rt = rt * 8 + (int)(blockIdx.x & 7);
-  return rt < a.row_tiles;
-}
+// The tiles of a workgroup.  Workgroups go round the 8 XCDs, each with an L2 of its own; what runs on an XCD at one time should
+// share rows and weights.  Its tiles are taken in the order "four output tiles across, row tiles down", one workgroup the next
+// to its neighbour's: with eight row tiles or more an XCD has every eighth of them, else a contiguous piece of that order.
+struct RingOrder {
+  u32 rows, out_tiles, base, count;   // row tiles in the order, tiles before and in this XCD's piece
+  bool deal;
+  __device__ __forceinline__ RingOrder(const RingArgs &a, u32 row_tiles) : out_tiles((u32)a.out_tiles), deal(row_tiles >= 8) {
+    const u32 xcd = blockIdx.x & 7;
+    rows = deal ? (row_tiles - xcd + 7) / 8 : row_tiles;
+    const u32 total = out_tiles * rows, per = (total + 7) / 8;
+    base = deal ? 0 : xcd * per;
+    count = deal ? total : base >= total ? 0 : total - base < per ? total - base : per;
+  }
+  __device__ __forceinline__ void tile(u32 i, int &ot, u32 &rt) const {
+    const u32 q = base + i, panel = q / (4 * rows), rest = q - panel * 4 * rows;
+    const u32 wide = out_tiles - panel * 4 < 4 ? out_tiles - panel * 4 : 4;
+    rt = rest / wide, ot = (int)(panel * 4 + rest % wide);
+    if (deal) rt = rt * 8 + (blockIdx.x & 7);
+  }
+};
 
 // the row of x that row r reads, or -1 (an index outside [0, n_tokens) reads as a row of zeros)
 __device__ __forceinline__ long long ring_token(const RingArgs &a, size_t r) {
@@ -212,10 +244,13 @@ template <int NX, int NW, int WK>
 __global__ __launch_bounds__(64 * WK, 2) void ring_rows_kernel(RingArgs a) {
   __shared__ uint4 lds[WK][512];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  int g;
-  size_t lo, hi;
   if (blockIdx.y == 0) ring_zero_rest(a, (int)blockIdx.x * 32, (int)blockIdx.x * 32 + 32);
-  if (!ring_find_tile<32>(a, blockIdx.y, g, lo, hi)) return;
+  RingGroups<32> groups;
+  RingTile tile;
+  if (a.offsets) groups.load(a, 0);
+  if (!ring_find_tile(a, groups, blockIdx.y, tile)) return;
+  const int g = tile.g;
+  const size_t lo = tile.lo, hi = tile.hi;
   const int ot = (int)blockIdx.x, r = lane & 15, sub = lane >> 4;
   const RingRow row[2] = {ring_row(a, lo + r, hi), ring_row(a, lo + 16 + r, hi)};
   const int8_t *pw = a.w + ((size_t)g * a.out32 + ot) * a.k32 * (NW * 1024) + lane * 16;
@@ -275,9 +310,12 @@ __global__ __launch_bounds__(1024) void ring_few_kernel(RingArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int ot = (int)blockIdx.x;   // 16 outputs
   if (blockIdx.y == 0) ring_zero_rest(a, ot * 16, ot * 16 + 16);
-  int g;
-  size_t lo, hi;
-  if (!ring_find_tile<8>(a, blockIdx.y, g, lo, hi)) return;
+  RingGroups<8> groups;
+  RingTile tile;
+  if (a.offsets) groups.load(a, 0);
+  if (!ring_find_tile(a, groups, blockIdx.y, tile)) return;
+  const int g = tile.g;
+  const size_t lo = tile.lo, hi = tile.hi;
   // a lane cuts four words of rows lane % 4 and, with more than four rows, lane % 4 + 4
   const int r = lane & 3, k4 = lane >> 2;
   const bool eight = hi - lo > 4;
@@ -369,24 +407,40 @@ template <int NX, int NW, int OT, bool TWO>
 __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
   __shared__ uint4 xs[3][2 * NX * 64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  int g, ot, rt;
-  size_t lo, hi;
-  if (!ring_block(a, ot, rt)) return;
-  if (rt == 0 && !a.ws) ring_zero_rest(a, ot * 256 * OT, (ot + 1) * 256 * OT);
-  if (!ring_find_tile<32>(a, rt, g, lo, hi)) return;
-  const int ot0 = (ot * 8 + wave) * OT;
   const int r = lane & 15, sub = lane >> 4;
+  RingGroups<32> groups;
+  if (a.offsets) groups.load(a, 0);
+  const RingOrder order(a, ring_count_tiles(a, groups));
+  if (!a.ws)
+    for (int t = (int)blockIdx.x; t < a.out_tiles; t += gridDim.x) ring_zero_rest(a, t * 256 * OT, (t + 1) * 256 * OT);
+  const int last = a.k32 / 2 - 1;
+  const int first = (int)((long long)(last + 1) * blockIdx.y / gridDim.y);
+  const int end = (int)((long long)(last + 1) * (blockIdx.y + 1) / gridDim.y);
+
+  u32 rt;
+  RingTile tile;
+  if (blockIdx.x >> 3 >= order.count) return;
+  order.tile(blockIdx.x >> 3, tile.ot, rt);
+  if (!ring_find_tile(a, groups, rt, tile)) return;
+  const size_t lo = tile.lo, hi = tile.hi;
+  const int ot0 = (tile.ot * 8 + wave) * OT;
   // this wave cuts the 16 x 16 block (row half wave % 2, column quarter wave / 2) of every step
   const size_t my_row = lo + (wave & 1) * 16 + r;
   const long long my_token = my_row < hi ? ring_token(a, my_row) : -1;
   const size_t token = my_token < 0 ? 0 : (size_t)my_token;   // any row will do: its sums are not used
   const int in_step = (wave >> 1) * 16 + sub * 4;
   const u64 *px = a.x + token * a.ldx + in_step, *px1 = TWO ? a.x1 + token * a.ldx1 + in_step : nullptr;
+  const int8_t *pw[OT];
+#pragma unroll
+  for (int o = 0; o < OT; ++o) {
+    const int n = ot0 + o < a.out32 ? ot0 + o : a.out32 - 1;
+    pw[o] = a.w + ((size_t)tile.g * a.out32 + n) * a.k32 * (NW * 1024);
+  }
+
   struct Words {
     u64 x[4], x1[TWO ? 4 : 1];
   };
   Words words[2];
-  const int last = a.k32 / 2 - 1;
   auto load_x = [&](Words &v, int c) {
     c = c < last ? c : last;
     const int k = c * 64 < a.cols - 64 ? c * 64 : a.cols - 64;   // the last step ends with the last column
@@ -406,12 +460,6 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
     for (int k = 0; k < 4; ++k)
       if (4 * half + k < NX) reinterpret_cast<u32 *>(frag + (4 * half + k) * 64)[sub] = d[k] ^ lo32(kDigitBias);
   };
-  const int8_t *pw[OT];
-#pragma unroll
-  for (int o = 0; o < OT; ++o) {
-    const int t = ot0 + o < a.out32 ? ot0 + o : a.out32 - 1;
-    pw[o] = a.w + ((size_t)g * a.out32 + t) * a.k32 * (NW * 1024);
-  }
   v4i w[2][2][OT][NW];
   v16i acc[OT][NX];
   auto load_w = [&](int p, int h, int c) {
@@ -427,9 +475,11 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
   v4i f[D + 1];
   // the barrier orders LDS alone: loads from memory stay in flight across it
   auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-  // Step c (p = c % 2): products from buffer rd, digits of step c + 2 into wr.  The barrier in its middle publishes them; the
-  // buffer they replace was read a step ago, before that step's barrier or right after it, never behind this one.
-  constexpr int kCut = NX <= 5 ? 1 : NX - 4;
+  // Step c: products from buffer rd, digits of step c + 2 into wr, words and weights of set p.  All waves have read the last of
+  // wr, the buffer of step c - 1, when they reach this step's barrier, so it is written behind it; the next step's barrier
+  // publishes the digits, before the end of that step starts to read them.
+  constexpr int kBarrier = NX / 2, kCut = kBarrier + 1;
+  static_assert(kCut + 2 < 2 * NX && kBarrier < 2 * NX - D, "cut within the step, read ahead behind the barrier");
   int rd = 0, nx = 1, wr = 2;
   // Products, reads and the cutting of digits are kept in this order (sched_barrier): moved together, the cutting would wait
   // for words that were only just asked for, and reads for products.
@@ -444,23 +494,19 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
         for (int j = 0; j < NW; ++j)
           if (i + j < NX)
             acc[o][i + j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[p][h][o][j], f[t % (D + 1)], acc[o][i + j], 0, 0, 0);
+      if (t == kBarrier) barrier();
       if (t == kCut) store_x(words[p], wr, 0);
       if (NX > 4 && t == kCut + 2) store_x(words[p], wr, 1);
-      if (t == NX - 1) {
-        load_x(words[p], c + 4);
-        load_w(p, 0, c + 2);
-        barrier();
-      }
+      if (t == NX - 1) load_w(p, 0, c + 2);
       __builtin_amdgcn_sched_barrier(0x4);   // scalar arithmetic may cross
     }
+    load_x(words[p], c + 4);
     load_w(p, 1, c + 2);
     const int t = rd;
     rd = nx, nx = wr, wr = t;
     __builtin_amdgcn_sched_barrier(0x4);
   };
   constexpr int kFlush = 131071 / NW / 64;   // steps whose sums fit 32 bits
-  const int first = (int)((long long)(last + 1) * blockIdx.y / gridDim.y);
-  const int end = (int)((long long)(last + 1) * (blockIdx.y + 1) / gridDim.y);
   for (int c0 = first; c0 < end; c0 += kFlush) {
     const int c1 = c0 + kFlush < end ? c0 + kFlush : end;
     Words one, two;
@@ -470,6 +516,7 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
     for (int p = 0; p < 2; ++p) load_w(p, 0, c0 + p), load_w(p, 1, c0 + p);
     load_x(words[0], c0 + 2);
     load_x(words[1], c0 + 3);
+    barrier();   // the last segment's digits have been read
 #pragma unroll
     for (int half = 0; half < (NX > 4 ? 2 : 1); ++half) store_x(one, rd, half), store_x(two, nx, half);
 #pragma unroll
@@ -512,18 +559,34 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
   }
 }
 
-// the parts of k that several workgroups summed: out = add + sum of the parts
+// the parts of k that several workgroups summed: out = add + sum of the parts, two outputs a lane, four parts asked for at once
 __global__ __launch_bounds__(256) void ring_join_kernel(RingArgs a, int parts) {
-  const int n = (int)(blockIdx.x * 256 + threadIdx.x);
+  const int n = (int)(blockIdx.x * 256 + threadIdx.x) * 2;
   const size_t row = blockIdx.y;
   if (n >= a.n_out) return;
+  const bool pair = n + 1 < a.n_out;
+  u64 *out = a.out + row * a.ldo + n;
+  u64 v[2] = {0, 0};
   if (a.offsets && ((long long)row < a.offsets[0] || (long long)row >= a.offsets[a.groups])) {
-    if (a.zero_rest) a.out[row * a.ldo + n] = 0;
-    return;
+    if (!a.zero_rest) return;
+  } else {
+    const u64 *ws = a.ws + row * a.n_out + n;
+    const size_t stride = a.n_rows * a.n_out;
+    for (int p = 0; p < parts; p += 4) {
+      u64 u[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u64 *q = ws + (p + i < parts ? p + i : p) * stride;
+        u[i][0] = q[0], u[i][1] = q[pair];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (p + i < parts) v[0] += u[i][0], v[1] += u[i][1];
+    }
+    if (a.add) v[0] += a.add[row * a.ldadd + n], v[1] += a.add[row * a.ldadd + n + pair];
   }
-  u64 v = a.add ? a.add[row * a.ldadd + n] : 0;
-  for (int p = 0; p < parts; ++p) v += a.ws[((size_t)p * a.n_rows + row) * a.n_out + n];
-  a.out[row * a.ldo + n] = v & a.mask;
+  out[0] = v[0] & a.mask;
+  if (pair) out[1] = v[1] & a.mask;
 }
 
 // ---- weights: how many digits the widest needs, then the layout
@@ -591,7 +654,7 @@ static int ring_parts(size_t tiles, size_t steps, int products, size_t outputs) 
   for (int p = 1; p <= 16 && (size_t)p * 2 <= std::max<size_t>(steps, 2); ++p) {
     const double rounds = (double)((tiles * p + 255) / 256);
     const double t = rounds * ((double)((steps + p - 1) / p) * step + 5) + (p > 1 ? 5 + p * (double)outputs * 16 / 4.5e6 : 0);
-    if (p == 1 || t < 0.95 * least) best = p, least = t;
+    if (p == 1 || t < 0.9 * least) best = p, least = t;
   }
   return best;
 }
@@ -619,12 +682,11 @@ static void ring_launch(RingArgs a, hipStream_t s) {
   if (parts == 1) a.ws = nullptr;
   const u64 mask = a.mask;
   if (a.ws) a.mask = ~u64(0);
-  const int blocks = a.row_tiles >= 8 ? (a.row_tiles + 7) / 8 * 8 * a.out_tiles : (a.row_tiles * a.out_tiles + 7) / 8 * 8;
-  const dim3 grid(blocks, parts);
+  const dim3 grid((a.row_tiles >= 8 ? (a.row_tiles + 7) / 8 * a.out_tiles : (a.row_tiles * a.out_tiles + 7) / 8) * 8, parts);
   if (a.x1) hipLaunchKernelGGL((ring_tile_kernel<NX, NW, OT, true>), grid, dim3(512), 0, s, a);
   else hipLaunchKernelGGL((ring_tile_kernel<NX, NW, OT, false>), grid, dim3(512), 0, s, a);
   a.mask = mask;
-  if (a.ws) hipLaunchKernelGGL(ring_join_kernel, dim3((a.n_out + 255) / 256, (unsigned)a.n_rows), dim3(256), 0, s, a, parts);
+  if (a.ws) hipLaunchKernelGGL(ring_join_kernel, dim3((a.n_out + 511) / 512, (unsigned)a.n_rows), dim3(256), 0, s, a, parts);
 }
 // digits of x and of the weights that kernels exist for (x: what the ring needs, rounded up; weights: 1..4 or all)
 static int ring_digits_x(int bw) { return bw <= 32 ? 4 : bw <= 40 ? 5 : bw <= 48 ? 6 : 8; }
