@@ -183,41 +183,6 @@ __device__ __forceinline__ void ring_digits4(const u64 (&v)[4], u32 (&dig)[8]) {
   }
 }
 
-// ---- the rows' digits.  A lane cuts four words of one row: block b of a step is 16 rows (b & 1 ...) x 16 columns, and in it
-// lane l takes row l % 16, columns 4 * (l / 16) ..; four lanes read 128 contiguous bytes, and the 64 dwords a block gives per
-// digit fall into 64 different LDS banks.
-struct RingRow {
-  const u64 *x, *x1;   // null: a row of zeros
-};
-__device__ __forceinline__ RingRow ring_row(const RingArgs &a, size_t row, size_t hi) {
-  const long long t = row < hi ? ring_token(a, row) : -1;
-  return RingRow{t < 0 ? nullptr : a.x + (size_t)t * a.ldx, t < 0 || !a.x1 ? nullptr : a.x1 + (size_t)t * a.ldx1};
-}
-__device__ __forceinline__ void ring_load_row(const RingArgs &a, const RingRow &p, int k, u64 (&v)[4], u64 (&u)[4]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = 0, u[e] = 0;
-  if (k + 4 <= a.cols) {
-    if (p.x) ring_load4(p.x + k, v);
-    if (p.x1) ring_load4(p.x1 + k, u);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (p.x && k + e < a.cols) v[e] = p.x[k + e];
-      if (p.x1 && k + e < a.cols) u[e] = p.x1[k + e];
-    }
-  }
-}
-// into the fragment of each digit: lane (k / 16) * 32 + row holds 16 columns of a row; frag points at digit 0's
-template <int NX>
-__device__ __forceinline__ void ring_store_digits(uint4 *frag, int row, int k16, int sub, const u64 (&v)[4], const u64 (&u)[4]) {
-  u64 t[4];
-  u32 dig[8];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) t[e] = v[e] + u[e];
-  ring_digits4<NX>(t, dig);
-#pragma unroll
-  for (int d = 0; d < NX; ++d) reinterpret_cast<u32 *>(&frag[d * 64 + k16 * 32 + row])[sub] = dig[d];
-}
 __device__ __forceinline__ v4i as_v4i(const uint4 &t) { return v4i{(int)t.x, (int)t.y, (int)t.z, (int)t.w}; }
 // sum_s 256^s acc_s mod 2^64: what lies at 2^32 and above in 32-bit arithmetic
 template <int NX, typename T>
@@ -231,78 +196,43 @@ __device__ __forceinline__ u64 ring_value(const T (&acc)[NX], int e) {
   return make64(lo32(v), h);
 }
 
-// first column of fragment c: steps of two fragments, the last of which ends with the last column (weights of columns that the
-// step before has already are laid out as zeros)
-__device__ __forceinline__ int ring_column(const RingArgs &a, int c) {
-  const int k = (c >> 1) * 64;
-  return (c >> 1) == a.k32 / 2 - 1 && a.cols > 64 ? a.cols - 64 + (c & 1) * 32 : k + (c & 1) * 32;
+// ---- which columns a step's 64 places hold: the last step ends with the last column, and with fewer than 64 columns so does the
+// last piece of four that a lane loads.  Nothing is read past a row's end; weights at places whose column an earlier place has
+// (or that there is none for) are laid out as zeros.
+__device__ __forceinline__ int ring_step_column(int cols, int c) {
+  const int k = c * 64;
+  return k + 64 <= cols ? k : cols < 64 ? 0 : cols - 64;
 }
+__device__ __forceinline__ int ring_piece(int cols, int place) { return cols < 64 && place + 4 > cols ? cols - 4 : place; }
 
-// Small products: one workgroup per 32 rows x 32 outputs, its WK waves split k in steps of 32 columns and join their 64-bit
-// sums through LDS.  Every wave cuts its own digits into LDS of its own, so the loop has no barrier.
-template <int NX, int NW, int WK>
-__global__ __launch_bounds__(64 * WK, 2) void ring_rows_kernel(RingArgs a) {
-  __shared__ uint4 lds[WK][512];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  if (blockIdx.y == 0) ring_zero_rest(a, (int)blockIdx.x * 32, (int)blockIdx.x * 32 + 32);
+// Fewer than 4 columns: 64-bit products, one output a lane.
+__global__ __launch_bounds__(256) void ring_narrow_kernel(RingArgs a, int nw) {
+  if (blockIdx.y == 0) ring_zero_rest(a, (int)blockIdx.x * 256, (int)blockIdx.x * 256 + 256);
   RingGroups<32> groups;
   RingTile tile;
   if (a.offsets) groups.load(a, 0);
   if (!ring_find_tile(a, groups, blockIdx.y, tile)) return;
-  const int g = tile.g;
-  const size_t lo = tile.lo, hi = tile.hi;
-  const int ot = (int)blockIdx.x, r = lane & 15, sub = lane >> 4;
-  const RingRow row[2] = {ring_row(a, lo + r, hi), ring_row(a, lo + 16 + r, hi)};
-  const int8_t *pw = a.w + ((size_t)g * a.out32 + ot) * a.k32 * (NW * 1024) + lane * 16;
-  v16i acc[NX];
-#pragma unroll
-  for (int s = 0; s < NX; ++s)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[s][e] = 0;
-  u64 xv[4][4], xu[4][4];
-  v4i w[NW];
-  auto load = [&](int c) {
-#pragma unroll
-    for (int j = 0; j < NW; ++j) w[j] = *reinterpret_cast<const v4i *>(pw + ((size_t)c * NW + j) * 1024);
-#pragma unroll
-    for (int b = 0; b < 4; ++b) ring_load_row(a, row[b & 1], ring_column(a, c) + (b >> 1) * 16 + sub * 4, xv[b], xu[b]);
-  };
-  if (wave < a.k32) load(wave);
-  for (int c = wave; c < a.k32; c += WK) {
-#pragma unroll
-    for (int b = 0; b < 4; ++b) ring_store_digits<NX>(lds[wave], (b & 1) * 16 + r, b >> 1, sub, xv[b], xu[b]);
-    v4i wc[NW];
-#pragma unroll
-    for (int j = 0; j < NW; ++j) wc[j] = w[j];
-    if (c + WK < a.k32) load(c + WK);
-#pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      const v4i x = as_v4i(lds[wave][i * 64 + lane]);
-#pragma unroll
-      for (int j = 0; j < NW; ++j)
-        if (i + j < NX) acc[i + j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wc[j], x, acc[i + j], 0, 0, 0);
-    }
+  const int n = (int)(blockIdx.x * 256 + threadIdx.x);
+  if (n >= a.n_out) return;
+  u64 w[3];
+  for (int k = 0; k < a.cols; ++k) {
+    w[k] = 0;
+    for (int j = 0; j < nw; ++j)
+      w[k] += (u64)(long long)a.w[(((size_t)tile.g * a.out32 + (n >> 5)) * a.k32 * nw + j) * 1024 + (n & 31) * 16 + k] << (8 * j);
   }
-  // element e of a lane: row lane % 32, output e % 4 + 8 * (e / 4) + 4 * (lane / 32)
-  u64 *part = reinterpret_cast<u64 *>(lds[wave]);
-#pragma unroll
-  for (int e = 0; e < 16; ++e) part[e * 64 + lane] = ring_value<NX>(acc, e);
-  __syncthreads();
-  for (int i = (int)threadIdx.x; i < 1024; i += 64 * WK) {
-    const int o = i & 31, rr = i >> 5, n = ot * 32 + o;
-    if (lo + rr >= hi || n >= a.n_out) continue;
-    const int at = ((o & 3) + 4 * (o >> 3)) * 64 + (o >> 2 & 1) * 32 + rr;
-    u64 v = a.add ? a.add[(lo + rr) * a.ldadd + n] : 0;
-#pragma unroll
-    for (int k = 0; k < WK; ++k) v += reinterpret_cast<const u64 *>(lds[k])[at];
-    a.out[(lo + rr) * a.ldo + n] = v & a.mask;
+  for (size_t row = tile.lo; row < tile.hi; ++row) {
+    const long long t = ring_token(a, row);
+    u64 v = a.add ? a.add[row * a.ldadd + n] : 0;
+    for (int k = 0; k < a.cols && t >= 0; ++k)
+      v += (a.x[(size_t)t * a.ldx + k] + (a.x1 ? a.x1[(size_t)t * a.ldx1 + k] : 0)) * w[k];
+    a.out[row * a.ldo + n] = v & a.mask;
   }
 }
 
 // Up to 8 rows: a workgroup computes them for 16 outputs, its 16 waves split k in steps of 64 columns and join their 64-bit sums
 // through LDS.  Bound by latency: everything a wave needs of its first steps is asked for at once (kAhead steps), and it cuts
 // its own digits into LDS of its own, so the loop has no barrier.  16 x 16 products (v_mfma_i32_16x16x64_i8), of whose rows 8
-// stay zero: their rate does not matter here, their few registers do.  Needs 64 columns or more.
+// stay zero: their rate does not matter here, their few registers do.  4 columns or more.
 template <int NX, int NW, bool TWO>
 __global__ __launch_bounds__(1024) void ring_few_kernel(RingArgs a) {
   constexpr int W = 16, kAhead = NW <= 2 && !TWO ? 2 : 1;
@@ -325,7 +255,8 @@ __global__ __launch_bounds__(1024) void ring_few_kernel(RingArgs a) {
     const size_t row = lo + 4 * b + r;
     const long long t = row < hi ? ring_token(a, row) : -1;
     const size_t token = t < 0 ? 0 : (size_t)t;   // any row will do: its sums are not used
-    px[b] = a.x + token * a.ldx + k4 * 4, px1[b] = TWO ? a.x1 + token * a.ldx1 + k4 * 4 : nullptr;
+    const int piece = ring_piece(a.cols, k4 * 4);
+    px[b] = a.x + token * a.ldx + piece, px1[b] = TWO ? a.x1 + token * a.ldx1 + piece : nullptr;
   }
   // 16 outputs x 64 columns of a step's two fragments: lane (quarter, output) reads 16 columns
   const int8_t *pw = a.w + ((size_t)g * a.out32 + (ot >> 1)) * a.k32 * (NW * 1024) + (lane >> 5) * (NW * 1024) +
@@ -337,7 +268,7 @@ __global__ __launch_bounds__(1024) void ring_few_kernel(RingArgs a) {
   } s[kAhead];
   auto load = [&](Step &v, int c) {
     c = c < last ? c : last;
-    const int k = c * 64 < a.cols - 64 ? c * 64 : a.cols - 64;   // the last step ends with the last column
+    const int k = ring_step_column(a.cols, c);
 #pragma unroll
     for (int j = 0; j < NW; ++j) v.w[j] = *reinterpret_cast<const v4i *>(pw + ((size_t)2 * c * NW + j) * 1024);
 #pragma unroll
@@ -402,7 +333,7 @@ __global__ __launch_bounds__(1024) void ring_few_kernel(RingArgs a) {
 // Large products: a workgroup of 8 waves computes 32 rows x 256*OT outputs in steps of 64 columns.  The rows' digits are cut
 // once per workgroup into LDS (three buffers, one barrier per step); the weights' fragments come straight from L2 in the order
 // they were laid out in.  Words and weights are loaded into registers two steps before they are used; nothing in the loop
-// branches.  Needs 64 columns or more.
+// branches.  4 columns or more.
 template <int NX, int NW, int OT, bool TWO>
 __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
   __shared__ uint4 xs[3][2 * NX * 64];
@@ -428,7 +359,7 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
   const size_t my_row = lo + (wave & 1) * 16 + r;
   const long long my_token = my_row < hi ? ring_token(a, my_row) : -1;
   const size_t token = my_token < 0 ? 0 : (size_t)my_token;   // any row will do: its sums are not used
-  const int in_step = (wave >> 1) * 16 + sub * 4;
+  const int in_step = ring_piece(a.cols, (wave >> 1) * 16 + sub * 4);
   const u64 *px = a.x + token * a.ldx + in_step, *px1 = TWO ? a.x1 + token * a.ldx1 + in_step : nullptr;
   const int8_t *pw[OT];
 #pragma unroll
@@ -443,7 +374,7 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
   Words words[2];
   auto load_x = [&](Words &v, int c) {
     c = c < last ? c : last;
-    const int k = c * 64 < a.cols - 64 ? c * 64 : a.cols - 64;   // the last step ends with the last column
+    const int k = ring_step_column(a.cols, c);
     ring_load4(px + k, v.x);
     if constexpr (TWO) ring_load4(px1 + k, v.x1);
   };
@@ -605,7 +536,11 @@ __global__ __launch_bounds__(256) void ring_weight_digits_kernel(const T *__rest
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) m = max(m, __shfl_xor(m, d));
-  if ((threadIdx.x & 63) == 0) atomicMax(need, m);
+  __shared__ int waves[4];
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = max(max(waves[0], waves[1]), max(waves[2], waves[3]));
+  if (threadIdx.x == 0 && *(volatile int *)need < m) atomicMax(need, m);
 }
 template <typename T>
 __global__ __launch_bounds__(256) void ring_weight_layout_kernel(const T *__restrict__ w, size_t rows, size_t cols, int bw,
@@ -614,15 +549,15 @@ __global__ __launch_bounds__(256) void ring_weight_layout_kernel(const T *__rest
   const size_t u = (size_t)blockIdx.x * 256 + threadIdx.x;   // (group, out32, k32, half, output): 16 columns of a row
   if (u >= n_units) return;
   const size_t frag = u >> 6, c = frag % k32, ot = frag / k32 % out32, g = frag / k32 / out32;
-  // columns as ring_column has them: the last step of 64 ends with the last column and skips what the step before has
-  const size_t step = c >> 1, start = step == k32 / 2 - 1 && cols > 64 ? cols - 64 : step * 64;
-  const size_t o = ot * 32 + (u & 31), k = start + (c & 1) * 32 + (u >> 5 & 1) * 16;
+  const size_t step = c >> 1, o = ot * 32 + (u & 31), place = (c & 1) * 32 + (u >> 5 & 1) * 16;
   u64 t[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const bool in = o < rows && k + e < cols && k + e >= step * 64;
+    const size_t piece = (place + e) & ~size_t(3);
+    const size_t k = cols < 4 ? place + e : ring_step_column((int)cols, (int)step) + ring_piece((int)cols, (int)piece) + (e & 3);
+    const bool in = o < rows && k < cols && k >= step * 64 && (cols >= 64 || k >= piece);
     const u64 C = 0x8080808080808080ull;
-    t[e] = ((u64)(in ? ring_weight(w, (g * rows + o) * cols + k + e, bw) : 0) + C) ^ C;
+    t[e] = ((u64)(in ? ring_weight(w, (g * rows + o) * cols + k, bw) : 0) + C) ^ C;
   }
   for (int j = 0; j < nw; ++j) {
     u32 d[4] = {0, 0, 0, 0};
@@ -634,7 +569,7 @@ __global__ __launch_bounds__(256) void ring_weight_layout_kernel(const T *__rest
 
 template <typename T>
 static void ring_launch_digits(const void *w, size_t n, int bw, int *need, hipStream_t s) {
-  hipLaunchKernelGGL(ring_weight_digits_kernel<T>, dim3((unsigned)std::min<size_t>((n + 255) / 256, 4096)), dim3(256), 0, s,
+  hipLaunchKernelGGL(ring_weight_digits_kernel<T>, dim3((unsigned)std::min<size_t>((n + 255) / 256, 2048)), dim3(256), 0, s,
                      (const T *)w, n, bw, need);
 }
 template <typename T>
@@ -659,7 +594,7 @@ static int ring_parts(size_t tiles, size_t steps, int products, size_t outputs) 
   return best;
 }
 // up to 8 rows in all go to ring_few_kernel, whose waves must not sum more columns than fit 32 bits
-static bool ring_few(size_t n_rows, size_t cols, int nw) { return n_rows <= 8 && cols >= 64 && (cols / 64 / 16 + 1) * 64 * nw <= 131071; }
+static bool ring_few(size_t n_rows, size_t cols, int nw) { return n_rows <= 8 && (cols / 64 / 16 + 1) * 64 * nw <= 131071; }
 static constexpr int ring_products(int nx, int nw) { return 2 * (nx * nw - nw * (nw - 1) / 2); }   // of a 64-column step
 // 32-output tiles a wave computes: the accumulators of one take 16 nx registers; two while they fit, for fewer digit reads
 static constexpr int ring_outputs(int nx, int nw) { return nx * 32 + nw * 32 <= 160 ? 2 : 1; }
@@ -674,10 +609,6 @@ static void ring_launch(RingArgs a, hipStream_t s) {
     return;
   }
   a.out_tiles = (a.out32 + 8 * OT - 1) / (8 * OT);
-  if (a.cols < 64) {
-    hipLaunchKernelGGL((ring_rows_kernel<NX, NW, 8>), dim3(a.out32, a.row_tiles), dim3(512), 0, s, a);
-    return;
-  }
   const int parts = !a.ws ? 1 : ring_parts((size_t)a.out_tiles * a.row_tiles, a.k32 / 2, OT * ring_products(NX, NW), a.n_rows * a.n_out);
   if (parts == 1) a.ws = nullptr;
   const u64 mask = a.mask;
@@ -789,7 +720,7 @@ static size_t ring_row_tiles(const mmh_ring_weights *w, size_t n_rows, bool offs
 }
 static size_t ring_ws_words(const mmh_ring_weights *w, size_t n_rows, size_t row_tiles) {
   const int ot = 8 * ring_outputs(w->nx, w->nw);
-  const int parts = w->cols < 64 || ring_few(n_rows, w->cols, w->nw) ? 1 : ring_parts(row_tiles * ((w->out32 + ot - 1) / ot), w->k32 / 2, ot / 8 * ring_products(w->nx, w->nw), n_rows * w->rows);
+  const int parts = w->cols < 4 || ring_few(n_rows, w->cols, w->nw) ? 1 : ring_parts(row_tiles * ((w->out32 + ot - 1) / ot), w->k32 / 2, ot / 8 * ring_products(w->nx, w->nw), n_rows * w->rows);
   return parts > 1 ? parts * n_rows * w->rows : 0;
 }
 }  // namespace mmh
@@ -823,8 +754,9 @@ extern "C" int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, s
   a.row_tiles = (int)ring_row_tiles(w, n_rows, d_offsets != nullptr);
   a.ws = d_ws && ws_words >= ring_ws_words(w, n_rows, a.row_tiles) ? d_ws : nullptr;
   hipStream_t s = (hipStream_t)stream;
-  bool ok = false;
-  if (w->nx == 4) ok = ring_dispatch_w<4>(w->nw, a, s);
+  bool ok = w->cols < 4;
+  if (ok) hipLaunchKernelGGL(ring_narrow_kernel, dim3((a.n_out + 255) / 256, a.row_tiles), dim3(256), 0, s, a, w->nw);
+  else if (w->nx == 4) ok = ring_dispatch_w<4>(w->nw, a, s);
   else if (w->nx == 5) ok = ring_dispatch_w<5>(w->nw, a, s);
   else if (w->nx == 6) ok = ring_dispatch_w<6>(w->nw, a, s);
   else if (w->nx == 8) ok = ring_dispatch_w<8>(w->nw, a, s);

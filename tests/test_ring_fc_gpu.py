@@ -61,8 +61,9 @@ def digits_of(w, bw):
 
 
 # one group: few and many rows, sizes around the tiles' 16 outputs and 64 columns, every ring's digit count and weight type
-@pytest.mark.parametrize("tokens", [1, 15, 16, 17, 70])
-@pytest.mark.parametrize("cols,rows", [(1, 1), (63, 15), (64, 16), (65, 17), (130, 300)])
+@pytest.mark.parametrize("tokens", [1, 4, 5, 8, 9, 31, 32, 33, 70])
+@pytest.mark.parametrize("cols,rows", [(1, 1), (3, 300), (4, 16), (5, 31), (6, 32), (33, 33), (63, 15), (64, 16), (65, 17), (127, 256), (130, 300),
+                                       (700, 257)])
 def test_sizes(mm, tokens, cols, rows):
     w = weights(SEED + rows, (1, rows, cols), np.int16)
     x = words(SEED + cols, (tokens, cols))
