@@ -120,6 +120,16 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 
 static u64 bw_mask_host(int bw) { return bw >= 64 ? ~u64(0) : (u64(1) << bw) - 1; }
 
+// Tokens and heads of a workgroup.  Small heads: several tokens, up to 4096 words and 2048 pairs of coefficients.  Few tokens:
+// the heads over several workgroups, each of 512 words or more, until there are 512 of them.
+static void rotary_blocks(size_t tokens, size_t heads, size_t dim, int half, int &per_tokens, int &per_heads) {
+  const size_t words = heads * dim;
+  size_t t = std::min<size_t>(4096 / words, 2048 / std::max(half, 1));
+  t = std::max<size_t>(1, std::min(t, tokens / 512));
+  size_t split = std::max<size_t>(1, std::min({512 / ((tokens + t - 1) / t), words / 512, heads}));
+  per_tokens = (int)t, per_heads = (int)((heads + split - 1) / split);
+}
+
 static int rotary_call(const uint64_t *d_x, size_t xs_token, size_t xs_head, size_t n_tokens, size_t n_heads, size_t head_dim,
                        const int64_t *d_pos, const uint64_t *d_phase, size_t rot_dim, int interleaved, double amplitude,
                        int frac_bits, int bw, u64 offset, u64 cmp_flip, uint64_t *d_out, uint64_t *d_cmp, size_t os_token,
@@ -138,7 +148,7 @@ static int rotary_call(const uint64_t *d_x, size_t xs_token, size_t xs_head, siz
   a.heads = (int)n_heads, a.dim = (int)head_dim, a.half = (int)rot_dim / 2, a.frac = frac_bits;
   a.scale = amplitude * (double)(u64(1) << frac_bits);
   a.mask = bw_mask_host(bw), a.offset = offset, a.cmp_flip = cmp_flip;
-  a.tokens_per_block = 1, a.heads_per_block = (int)n_heads;
+  rotary_blocks(n_tokens, n_heads, head_dim, a.half, a.tokens_per_block, a.heads_per_block);
   const dim3 grid((unsigned)((n_tokens + a.tokens_per_block - 1) / a.tokens_per_block),
                   (unsigned)((n_heads + a.heads_per_block - 1) / a.heads_per_block));
   const size_t lds = (size_t)std::max(1, a.tokens_per_block * a.half) * sizeof(int2);
