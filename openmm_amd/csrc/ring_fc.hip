@@ -496,31 +496,32 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
 // the parts of k that several workgroups summed: out = add + sum of the parts, two outputs a lane, four parts asked for at once
 __global__ __launch_bounds__(256) void ring_join_kernel(RingArgs a, int parts) {
   const int n = (int)(blockIdx.x * 256 + threadIdx.x) * 2;
-  const size_t row = blockIdx.y;
   if (n >= a.n_out) return;
   const bool pair = n + 1 < a.n_out;
-  u64 *out = a.out + row * a.ldo + n;
-  u64 v[2] = {0, 0};
-  if (a.offsets && ((long long)row < a.offsets[0] || (long long)row >= a.offsets[a.groups])) {
-    if (!a.zero_rest) return;
-  } else {
-    const u64 *ws = a.ws + row * a.n_out + n;
-    const size_t stride = a.n_rows * a.n_out;
-    for (int p = 0; p < parts; p += 4) {
-      u64 u[4][2];
+  const size_t stride = a.n_rows * a.n_out;
+  for (size_t row = blockIdx.y; row < a.n_rows; row += gridDim.y) {
+    u64 v[2] = {0, 0};
+    if (a.offsets && ((long long)row < a.offsets[0] || (long long)row >= a.offsets[a.groups])) {
+      if (!a.zero_rest) continue;
+    } else {
+      const u64 *ws = a.ws + row * a.n_out + n;
+      for (int p = 0; p < parts; p += 4) {
+        u64 u[4][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const u64 *q = ws + (p + i < parts ? p + i : p) * stride;
-        u[i][0] = q[0], u[i][1] = q[pair];
+        for (int i = 0; i < 4; ++i) {
+          const u64 *q = ws + (p + i < parts ? p + i : p) * stride;
+          u[i][0] = q[0], u[i][1] = q[pair];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (p + i < parts) v[0] += u[i][0], v[1] += u[i][1];
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (p + i < parts) v[0] += u[i][0], v[1] += u[i][1];
+      if (a.add) v[0] += a.add[row * a.ldadd + n], v[1] += a.add[row * a.ldadd + n + pair];
     }
-    if (a.add) v[0] += a.add[row * a.ldadd + n], v[1] += a.add[row * a.ldadd + n + pair];
+    u64 *out = a.out + row * a.ldo + n;
+    out[0] = v[0] & a.mask;
+    if (pair) out[1] = v[1] & a.mask;
   }
-  out[0] = v[0] & a.mask;
-  if (pair) out[1] = v[1] & a.mask;
 }
 
 // ---- weights: how many digits the widest needs, then the layout
@@ -584,9 +585,9 @@ static void ring_launch_layout(const void *w, const mmh_ring_weights *h, hipStre
 
 // Parts of k for `tiles` workgroups of the tile kernel on the chip's 256 compute units, by a model of its time (us): rounds of
 // workgroups, each with its steps and a start and end of its own, and the launch that adds up the parts, 16 bytes of traffic
-// per part and output.  A step of 30 products takes 2 us with all units busy, a few products no less than 1.
+// per part and output.  A step of 30 products takes 1.45 us with all units busy, one of a few products no less than 1.
 static int ring_parts(size_t tiles, size_t steps, int products, size_t outputs) {
-  const double step = std::max(1.0, products * (2.0 / 30));
+  const double step = std::max(1.0, products * (1.45 / 30));
   int best = 1;
   double least = 0;
   for (int p = 1; p <= 16 && (size_t)p * 2 <= std::max<size_t>(steps, 2); ++p) {
@@ -612,7 +613,8 @@ static void ring_launch(RingArgs a, hipStream_t s) {
     return;
   }
   a.out_tiles = (a.out32 + 8 * OT - 1) / (8 * OT);
-  const int parts = !a.ws ? 1 : ring_parts((size_t)a.out_tiles * a.row_tiles, a.k32 / 2, OT * ring_products(NX, NW), a.n_rows * a.n_out);
+  const size_t tiles = (size_t)a.out_tiles * a.row_tiles;
+  const int parts = !a.ws ? 1 : ring_parts(tiles, a.k32 / 2, OT * ring_products(NX, NW), a.n_rows * a.n_out);
   if (parts == 1) a.ws = nullptr;
   const u64 mask = a.mask;
   if (a.ws) a.mask = ~u64(0);
@@ -620,7 +622,7 @@ static void ring_launch(RingArgs a, hipStream_t s) {
   if (a.x1) hipLaunchKernelGGL((ring_tile_kernel<NX, NW, OT, true>), grid, dim3(512), 0, s, a);
   else hipLaunchKernelGGL((ring_tile_kernel<NX, NW, OT, false>), grid, dim3(512), 0, s, a);
   a.mask = mask;
-  if (a.ws) hipLaunchKernelGGL(ring_join_kernel, dim3((a.n_out + 511) / 512, (unsigned)a.n_rows), dim3(256), 0, s, a, parts);
+  if (a.ws) hipLaunchKernelGGL(ring_join_kernel, dim3((a.n_out + 511) / 512, (unsigned)std::min<size_t>(a.n_rows, 65535)), dim3(256), 0, s, a, parts);
 }
 // digits of x and of the weights that kernels exist for (x: what the ring needs, rounded up; weights: 1..4 or all)
 static int ring_digits_x(int bw) { return bw <= 32 ? 4 : bw <= 40 ? 5 : bw <= 48 ? 6 : 8; }
@@ -722,8 +724,10 @@ static size_t ring_row_tiles(const mmh_ring_weights *w, size_t n_rows, bool offs
   return offsets ? n_rows / 32 + std::min(w->groups, n_rows) : (n_rows + 31) / 32;
 }
 static size_t ring_ws_words(const mmh_ring_weights *w, size_t n_rows, size_t row_tiles) {
-  const int ot = 8 * ring_outputs(w->nx, w->nw);
-  const int parts = w->cols < 4 || ring_few(n_rows, w->cols, w->nw) ? 1 : ring_parts(row_tiles * ((w->out32 + ot - 1) / ot), w->k32 / 2, ot / 8 * ring_products(w->nx, w->nw), n_rows * w->rows);
+  if (w->cols < 4 || ring_few(n_rows, w->cols, w->nw)) return 0;
+  const int ot = ring_outputs(w->nx, w->nw);
+  const size_t tiles = row_tiles * ((w->out32 + 8 * ot - 1) / (8 * ot));
+  const int parts = ring_parts(tiles, w->k32 / 2, ot * ring_products(w->nx, w->nw), n_rows * w->rows);
   return parts > 1 ? parts * n_rows * w->rows : 0;
 }
 }  // namespace mmh
@@ -735,8 +739,8 @@ extern "C" int mmh_ring_matmul_workspace(const mmh_ring_weights *w, size_t n_row
 }
 extern "C" int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, size_t ldx, const uint64_t *d_x1, size_t ldx1,
                                size_t n_tokens, const int64_t *d_rows, const int64_t *d_offsets, size_t n_rows,
-                               const uint64_t *d_add, size_t ldadd, uint64_t *d_out, size_t ldo, int zero_rest, uint64_t *d_ws, size_t ws_words,
-                               void *stream) {
+                               const uint64_t *d_add, size_t ldadd, uint64_t *d_out, size_t ldo, int zero_rest,
+                               uint64_t *d_ws, size_t ws_words, void *stream) {
   MMH_REQUIRE(w, MMH_ERR_NULL_POINTER);
   DeviceScope scope(w->device);
   if (scope.rc) MMH_FAIL(scope.rc, "cannot make the weights' device current");
@@ -746,8 +750,9 @@ extern "C" int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, s
   MMH_REQUIRE(n_tokens >= 1 && (d_rows || n_rows <= n_tokens), MMH_ERR_DIM_MISMATCH);
   MMH_REQUIRE(ldx >= w->cols && (!d_x1 || ldx1 >= w->cols) && ldo >= w->rows, MMH_ERR_DIM_MISMATCH);
   MMH_REQUIRE(!d_add || ldadd == 0 || ldadd >= w->rows, MMH_ERR_DIM_MISMATCH);
-  // row tiles are the second dimension of the grid, which the hardware counts in 16 bits
+  // row tiles are the second dimension of a grid, which the hardware counts in 16 bits, and with the output tiles the first
   MMH_REQUIRE(n_rows <= (size_t(1) << 19) && w->groups <= 32767, MMH_ERR_OUT_BOUND);
+  MMH_REQUIRE((n_rows / 32 + w->groups + 8) * (w->out32 + 8) < (size_t(1) << 31), MMH_ERR_OUT_BOUND);
   RingArgs a;
   a.w = w->d, a.x = d_x, a.x1 = d_x1, a.add = d_add, a.rows = d_rows, a.offsets = d_offsets, a.out = d_out;
   a.ldx = ldx, a.ldx1 = ldx1, a.ldadd = ldadd, a.ldo = ldo, a.n_tokens = n_tokens, a.n_rows = n_rows;

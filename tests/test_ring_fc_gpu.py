@@ -181,6 +181,52 @@ def test_strides(mm, tokens, pad, shift):
     assert bool((buf == 77).all())      # nothing written between the rows
 
 
+# k over several workgroups, whose sums a second launch joins (a few rows against long columns), and the same without scratch
+@pytest.mark.parametrize("tokens,cols,rows", [(9, 2048, 40), (48, 1500, 300), (200, 4096, 33)])
+@pytest.mark.parametrize("bw,dtype,top", [(64, np.int16, 32639), (37, np.int8, None), (64, np.int32, 1 << 29)])
+def test_split_columns(mm, tokens, cols, rows, bw, dtype, top):
+    import torch
+    from openmm_amd.lib import check, load_library
+    f = fc(bw)
+    g, off = 3, np.array([0, tokens // 3, tokens // 3, tokens - 2])
+    w, x, x1 = weights(SEED, (g, rows, cols), dtype, top), words(SEED, (tokens, cols)), words(SEED + 1, (tokens, cols))
+    add = words(SEED + 2, (tokens, rows), bw)
+    idx = np.random.default_rng(SEED).integers(0, tokens, tokens)
+    idx[1] = -1
+    rw = f.encodeWeights(dev(w))
+    assert rw.workspace(tokens) > 0
+    want = product(x, w, bw, off, idx, x1, add)
+    args = dev(x), dev(x1), dev(idx), dev(off), dev(add)
+    y = f.matMul(rw, args[0], args[3], rows=args[2], share1=args[1], add=args[4])
+    assert np.array_equal(host(y), want)       # rows that no group has: zeros
+    keep = torch.full((tokens, rows), 5, dtype=torch.int64, device="cuda")
+    f.matMul(rw, args[0], args[3], rows=args[2], share1=args[1], add=args[4], out=keep)
+    assert np.array_equal(host(keep)[:off[-1]], want[:off[-1]]) and bool((keep[off[-1]:] == 5).all())
+    keep.fill_(5)
+    p = [C.c_void_p(a.data_ptr()) for a in args]
+    check(load_library().mmh_ring_matmul(rw.handle, p[0], cols, p[1], cols, tokens, p[2], p[3], tokens, p[4], rows,
+                                         C.c_void_p(keep.data_ptr()), rows, 0, None, 0, None))
+    assert np.array_equal(host(keep)[:off[-1]], want[:off[-1]]) and bool((keep[off[-1]:] == 5).all())
+
+
+def test_far_rows(mm):
+    """rows further apart than 32 bits count, in words as in bytes"""
+    import torch
+    cols, rows, bw, far = 70, 20, 64, (1 << 29) + 8
+    w = weights(SEED, (1, rows, cols), np.int16)
+    x = words(SEED, (10, cols))
+    f = fc(bw)
+    rw = f.encodeWeights(dev(w))
+    buf = torch.empty(9 * far + 128, dtype=torch.int64, device="cuda")     # 39 GB, of which ten rows are touched
+    wide = buf.as_strided((10, cols), (far, 1))
+    wide.copy_(dev(x))
+    assert np.array_equal(host(f.matMul(rw, wide)), product(x, w, bw))
+    assert np.array_equal(host(f.matMul(rw, wide[:5])), product(x[:5], w, bw))
+    out = buf.as_strided((10, rows), (far, 1), 100)
+    f.matMul(rw, dev(x), out=out)
+    assert np.array_equal(host(out.contiguous()), product(x, w, bw))
+
+
 def test_streams_and_replays(mm):
     """two calls at once on two streams; a captured call replayed among eager work"""
     import torch

@@ -104,6 +104,21 @@ def test_strides(mm, interleaved, dim, rot, shift, pad):
     assert np.array_equal(host(r.rotate(y, dev(pos))), want)
 
 
+def test_far_tokens(mm):
+    """tokens further apart than 32 bits count"""
+    import torch
+    from openmm_amd.rotary import Rotary, rotary_phases
+    far = (1 << 29) + 16
+    x, pos, ph = words(SEED, (9, 2, 16)), positions(SEED, 9), rotary_phases(16)
+    buf = torch.empty(8 * far + 64, dtype=torch.int64, device="cuda")     # 34 GB, of which nine rows are touched
+    wide = buf.as_strided((9, 2, 16), (far, 16, 1))
+    wide.copy_(dev(x))
+    r = Rotary(ph, 16, 12, 64)
+    want = rotary(x, pos, ph, 12, 64)
+    assert np.array_equal(host(r.rotate(wide, dev(pos))), want)
+    assert np.array_equal(host(r.rotate(wide, dev(pos), out=wide)), want)
+
+
 @pytest.mark.parametrize("party", [1, 2])
 @pytest.mark.parametrize("signed_arith", [True, False])
 @pytest.mark.parametrize("heuristic", [True, False])
@@ -159,6 +174,7 @@ def test_refusals(mm):
     import torch
     from openmm_amd.lib import MMHError
     from openmm_amd.rotary import Rotary, rotary_phases
+    from openmm_amd.truncation import Truncation
     ph = rotary_phases(16)
     r = Rotary(ph, 16, 12, 64)
     z = lambda *s: torch.zeros(s, dtype=torch.int64, device="cuda")
@@ -174,6 +190,7 @@ def test_refusals(mm):
         (3, lambda: r.rotate(x, z(3))), (7, lambda: r.rotate(x, pos.int())), (7, lambda: r.rotate(x, pos.cpu())),
         (7, lambda: r.rotate(x, z(8)[::2])), (3, lambda: r.rotate(x, pos, out=z(4, 3, 16))),
         (3, lambda: r.rotate(x, pos, out=z(1, 2, 16).expand(4, 2, 16))),      # rows of the result on top of each other
+        (7, lambda: Truncation(1, None).truncate_rotary(r, x, pos, 0)), (7, lambda: Truncation(2, None).truncate_rotary(r, x, pos, 62)),
         (7, lambda: r.truncate_pre(3, x, pos)), (7, lambda: Rotary(ph, 16, 0, 3).truncate_pre(1, x, pos)),
     ]
     for code, call in bad:
