@@ -393,7 +393,7 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
     for (int k = 0; k < 4; ++k)
       if (4 * half + k < NX) reinterpret_cast<u32 *>(frag + (4 * half + k) * 64)[sub] = d[k] ^ lo32(kDigitBias);
   };
-  constexpr int kSets = NW <= 4 ? 2 : 1;   // weights are loaded this many steps before their use (registers)
+  constexpr int kSets = NW <= (OT == 1 ? 4 : 5 - NX) ? 2 : 1;   // weights are loaded this many steps before their use (registers)
   v4i w[kSets][2][OT][NW];
   v16i acc[OT][NX];
   auto load_w = [&](int p, int h, int c) {
@@ -600,42 +600,68 @@ static int ring_parts(size_t tiles, size_t steps, int products, size_t outputs) 
 // up to 8 rows in all go to ring_few_kernel, whose waves must not sum more columns than fit 32 bits
 static bool ring_few(size_t n_rows, size_t cols, int nw) { return n_rows <= 8 && (cols / 64 / 16 + 1) * 64 * nw <= 131071; }
 static constexpr int ring_products(int nx, int nw) { return 2 * (nx * nw - nw * (nw - 1) / 2); }   // of a 64-column step
-// 32-output tiles a wave computes: the accumulators of one take 16 nx registers; two while they fit, for fewer digit reads
-static constexpr int ring_outputs(int nx, int nw) { return nx * 32 + nw * 32 <= 160 ? 2 : 1; }
+// 32-output tiles a wave computes.  Two halve the reads of digits from LDS, which bound the product when there are few digits,
+// and fit the registers (16 nx for the sums of each) for these; they pay when the chip has work enough: 4096 x 2048 x 2048 with
+// digits 4 x 1 135 -> 80 us, 4 x 2 135 -> 114, 5 x 1 121 -> 90, 6 x 1 121 -> 101, 5 x 2 155 -> 138, but 1024 rows 35 -> 39 us
+// (5 x 1), 40 -> 52 us (5 x 2).
+static constexpr bool ring_wide_fits(int nx, int nw, bool two) { return nx + nw <= 6 || (!two && nx + nw <= 7 && nw <= 2); }
+static size_t ring_out_tiles(size_t out32, int ot) { return (out32 + 8 * ot - 1) / (8 * ot); }
+static bool ring_wide(int nx, int nw, bool two, size_t out32, size_t row_tiles) {
+  return ring_wide_fits(nx, nw, two) && ring_out_tiles(out32, 2) * row_tiles >= 256;
+}
+// parts of k of a call (1: the tile kernel writes the result itself)
+static int ring_call_parts(int nx, int nw, bool two, size_t out32, size_t row_tiles, size_t steps, size_t outputs) {
+  const int ot = ring_wide(nx, nw, two, out32, row_tiles) ? 2 : 1;
+  return ring_parts(ring_out_tiles(out32, ot) * row_tiles, steps, ot * ring_products(nx, nw), outputs);
+}
 
-template <int NX, int NW>
+template <int NX, int NW, int OT, bool TWO>
+static void ring_launch_tiles(RingArgs a, hipStream_t s, int parts) {
+  a.out_tiles = (int)ring_out_tiles(a.out32, OT);
+  const dim3 grid((a.row_tiles >= 8 ? (a.row_tiles + 7) / 8 * a.out_tiles : (a.row_tiles * a.out_tiles + 7) / 8) * 8, parts);
+  hipLaunchKernelGGL((ring_tile_kernel<NX, NW, OT, TWO>), grid, dim3(512), 0, s, a);
+}
+template <int NX, int NW, bool TWO>
 static void ring_launch(RingArgs a, hipStream_t s) {
-  constexpr int OT = ring_outputs(NX, NW);
   if (ring_few(a.n_rows, a.cols, NW)) {
     const dim3 grid((a.n_out + 15) / 16, a.offsets ? std::min<unsigned>(a.groups, a.n_rows) : 1);
-    if (a.x1) hipLaunchKernelGGL((ring_few_kernel<NX, NW, true>), grid, dim3(1024), 0, s, a);
-    else hipLaunchKernelGGL((ring_few_kernel<NX, NW, false>), grid, dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((ring_few_kernel<NX, NW, TWO>), grid, dim3(1024), 0, s, a);
     return;
   }
-  a.out_tiles = (a.out32 + 8 * OT - 1) / (8 * OT);
-  const size_t tiles = (size_t)a.out_tiles * a.row_tiles;
-  const int parts = !a.ws ? 1 : ring_parts(tiles, a.k32 / 2, OT * ring_products(NX, NW), a.n_rows * a.n_out);
+  const int parts = a.ws ? ring_call_parts(NX, NW, TWO, a.out32, a.row_tiles, a.k32 / 2, a.n_rows * a.n_out) : 1;
   if (parts == 1) a.ws = nullptr;
   const u64 mask = a.mask;
   if (a.ws) a.mask = ~u64(0);
-  const dim3 grid((a.row_tiles >= 8 ? (a.row_tiles + 7) / 8 * a.out_tiles : (a.row_tiles * a.out_tiles + 7) / 8) * 8, parts);
-  if (a.x1) hipLaunchKernelGGL((ring_tile_kernel<NX, NW, OT, true>), grid, dim3(512), 0, s, a);
-  else hipLaunchKernelGGL((ring_tile_kernel<NX, NW, OT, false>), grid, dim3(512), 0, s, a);
+  if constexpr (ring_wide_fits(NX, NW, TWO)) {
+    if (ring_wide(NX, NW, TWO, a.out32, a.row_tiles)) ring_launch_tiles<NX, NW, 2, TWO>(a, s, parts);
+    else ring_launch_tiles<NX, NW, 1, TWO>(a, s, parts);
+  } else {
+    ring_launch_tiles<NX, NW, 1, TWO>(a, s, parts);
+  }
   a.mask = mask;
-  if (a.ws) hipLaunchKernelGGL(ring_join_kernel, dim3((a.n_out + 511) / 512, (unsigned)std::min<size_t>(a.n_rows, 65535)), dim3(256), 0, s, a, parts);
+  if (a.ws)
+    hipLaunchKernelGGL(ring_join_kernel, dim3((a.n_out + 511) / 512, (unsigned)std::min<size_t>(a.n_rows, 65535)), dim3(256), 0,
+                       s, a, parts);
 }
 // digits of x and of the weights that kernels exist for (x: what the ring needs, rounded up; weights: 1..4 or all)
 static int ring_digits_x(int bw) { return bw <= 32 ? 4 : bw <= 40 ? 5 : bw <= 48 ? 6 : 8; }
 static int ring_digits_w(int need, int nx) { return need <= 4 && need < nx ? need : nx; }
-template <int NX>
+template <int NX, bool TWO>
 static bool ring_dispatch_w(int nw, const RingArgs &a, hipStream_t s) {
-  if (nw == 1) ring_launch<NX, 1>(a, s);
-  else if (nw == 2) ring_launch<NX, 2>(a, s);
-  else if (nw == 3) ring_launch<NX, 3>(a, s);
-  else if (nw == 4) ring_launch<NX, 4>(a, s);
-  else if (nw == NX) ring_launch<NX, NX>(a, s);
+  if (nw == 1) ring_launch<NX, 1, TWO>(a, s);
+  else if (nw == 2) ring_launch<NX, 2, TWO>(a, s);
+  else if (nw == 3) ring_launch<NX, 3, TWO>(a, s);
+  else if (nw == 4) ring_launch<NX, 4, TWO>(a, s);
+  else if (nw == NX) ring_launch<NX, NX, TWO>(a, s);
   else return false;
   return true;
+}
+template <bool TWO>
+static bool ring_dispatch(int nx, int nw, const RingArgs &a, hipStream_t s) {
+  if (nx == 4) return ring_dispatch_w<4, TWO>(nw, a, s);
+  if (nx == 5) return ring_dispatch_w<5, TWO>(nw, a, s);
+  if (nx == 6) return ring_dispatch_w<6, TWO>(nw, a, s);
+  return nx == 8 && ring_dispatch_w<8, TWO>(nw, a, s);
 }
 }  // namespace mmh
 
@@ -723,18 +749,16 @@ namespace mmh {
 static size_t ring_row_tiles(const mmh_ring_weights *w, size_t n_rows, bool offsets) {
   return offsets ? n_rows / 32 + std::min(w->groups, n_rows) : (n_rows + 31) / 32;
 }
-static size_t ring_ws_words(const mmh_ring_weights *w, size_t n_rows, size_t row_tiles) {
+static size_t ring_ws_words(const mmh_ring_weights *w, size_t n_rows, size_t row_tiles, bool two) {
   if (w->cols < 4 || ring_few(n_rows, w->cols, w->nw)) return 0;
-  const int ot = ring_outputs(w->nx, w->nw);
-  const size_t tiles = row_tiles * ((w->out32 + 8 * ot - 1) / (8 * ot));
-  const int parts = ring_parts(tiles, w->k32 / 2, ot * ring_products(w->nx, w->nw), n_rows * w->rows);
+  const int parts = ring_call_parts(w->nx, w->nw, two, w->out32, row_tiles, w->k32 / 2, n_rows * w->rows);
   return parts > 1 ? parts * n_rows * w->rows : 0;
 }
 }  // namespace mmh
 extern "C" int mmh_ring_matmul_workspace(const mmh_ring_weights *w, size_t n_rows, size_t *words) {
   MMH_REQUIRE(w && words, MMH_ERR_NULL_POINTER);
-  // with offsets or without: the larger of the two
-  *words = std::max(ring_ws_words(w, n_rows, ring_row_tiles(w, n_rows, true)), ring_ws_words(w, n_rows, ring_row_tiles(w, n_rows, false)));
+  *words = 0;   // the most of what calls with or without offsets and a second share take
+  for (int i = 0; i < 4; ++i) *words = std::max(*words, ring_ws_words(w, n_rows, ring_row_tiles(w, n_rows, i & 1), i & 2));
   return MMH_OK;
 }
 extern "C" int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, size_t ldx, const uint64_t *d_x1, size_t ldx1,
@@ -760,14 +784,11 @@ extern "C" int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, s
   a.groups = (int)w->groups, a.cols = (int)w->cols, a.n_out = (int)w->rows, a.k32 = (int)w->k32, a.out32 = (int)w->out32;
   a.mask = w->bw >= 64 ? ~u64(0) : (u64(1) << w->bw) - 1;
   a.row_tiles = (int)ring_row_tiles(w, n_rows, d_offsets != nullptr);
-  a.ws = d_ws && ws_words >= ring_ws_words(w, n_rows, a.row_tiles) ? d_ws : nullptr;
+  a.ws = d_ws && ws_words >= ring_ws_words(w, n_rows, a.row_tiles, d_x1 != nullptr) ? d_ws : nullptr;
   hipStream_t s = (hipStream_t)stream;
   bool ok = w->cols < 4;
   if (ok) hipLaunchKernelGGL(ring_narrow_kernel, dim3((a.n_out + 255) / 256, a.row_tiles), dim3(256), 0, s, a, w->nw);
-  else if (w->nx == 4) ok = ring_dispatch_w<4>(w->nw, a, s);
-  else if (w->nx == 5) ok = ring_dispatch_w<5>(w->nw, a, s);
-  else if (w->nx == 6) ok = ring_dispatch_w<6>(w->nw, a, s);
-  else if (w->nx == 8) ok = ring_dispatch_w<8>(w->nw, a, s);
+  else ok = d_x1 ? ring_dispatch<true>(w->nx, w->nw, a, s) : ring_dispatch<false>(w->nx, w->nw, a, s);
   MMH_REQUIRE(ok, MMH_ERR_INTERNAL);
   MMH_HIP(hipGetLastError());
   return MMH_OK;

@@ -209,6 +209,20 @@ def test_split_columns(mm, tokens, cols, rows, bw, dtype, top):
     assert np.array_equal(host(keep)[:off[-1]], want[:off[-1]]) and bool((keep[off[-1]:] == 5).all())
 
 
+# many rows: tiles of twice the outputs for the digit counts that have them
+@pytest.mark.parametrize("two", [False, True])
+@pytest.mark.parametrize("cols", [40, 200])
+@pytest.mark.parametrize("bw,dtype", [(32, np.int8), (32, np.int16), (37, np.int8), (37, np.int16), (44, np.int8), (64, np.int8), (64, np.int16)])
+def test_many_rows(mm, bw, dtype, cols, two):
+    rows, tokens = 43, 8300
+    off = np.array([0, 17, 17, 8290])
+    w = weights(SEED, (3, rows, cols), dtype, None if dtype == np.int8 else 32639)
+    x, x1 = words(SEED, (tokens, cols)), words(SEED + 1, (tokens, cols)) if two else None
+    f = fc(bw)
+    y = f.matMul(f.encodeWeights(dev(w)), dev(x), dev(off), share1=dev(x1) if two else None)
+    assert np.array_equal(host(y), product(x, w, bw, off, None, x1))
+
+
 def test_far_rows(mm):
     """rows further apart than 32 bits count, in words as in bytes"""
     import torch
