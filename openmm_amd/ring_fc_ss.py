@@ -18,6 +18,10 @@ import torch
 from . import lib as L
 
 
+_INT64 = torch.int64
+_stream_of = torch._C._cuda_getCurrentRawStream
+
+
 def _need(cond, code, what):
     if not cond:
         raise L.MMHError(code, what)
@@ -25,7 +29,7 @@ def _need(cond, code, what):
 
 def _rows_of(t, what, cols, dev):
     """a 2-D int64 tensor on CUDA device ``dev`` with contiguous rows of ``cols`` words -> its row stride in words"""
-    if t.dtype is not torch.int64 or t.dim() != 2 or t.get_device() != dev:
+    if t.dtype is not _INT64 or t.dim() != 2 or t.get_device() != dev:
         raise L.MMHError(7, f"{what}: expected a 2-D int64 tensor on the weights' device")
     n, c = t.shape
     step, one = t.stride()
@@ -37,7 +41,7 @@ def _rows_of(t, what, cols, dev):
 
 
 def _index(t, what, dev):
-    if t.dtype is not torch.int64 or t.dim() != 1 or t.get_device() != dev or not t.is_contiguous():
+    if t.dtype is not _INT64 or t.dim() != 1 or t.get_device() != dev or not t.is_contiguous():
         raise L.MMHError(7, f"{what}: expected a contiguous 1-D int64 tensor on the weights' device")
     return t.shape[0]
 
@@ -134,7 +138,7 @@ class RingFCSS:
                 _need(add.shape[0] == n, 3, "matMul: add")
         new = out is None
         if new:
-            out, ldo = torch.empty((n, wide), dtype=torch.int64, device=x.device), wide
+            out, ldo = x.new_empty((n, wide)), wide
         else:
             ldo = _rows_of(out, "matMul: out", wide, dev)
             _need(out.shape[0] == n, 3, "matMul: out")
@@ -142,10 +146,10 @@ class RingFCSS:
             return out
         words = weights.workspace(n)
         if words:
-            ws = torch.empty(words, dtype=torch.int64, device=x.device)
+            ws = x.new_empty(words)
             pws = ws.data_ptr()
         rc = weights.lib.mmh_ring_matmul(weights.handle, x.data_ptr(), ldx, px1, ldx1, tokens, prows, poff, n, padd, ldadd,
-                                         out.data_ptr(), ldo, new, pws, words, torch._C._cuda_getCurrentRawStream(dev))
+                                         out.data_ptr(), ldo, new, pws, words, _stream_of(dev))
         if rc:
             L.check(rc)
         return out

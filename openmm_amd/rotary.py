@@ -13,6 +13,8 @@ from . import lib as L
 from .ring_fc_ss import _need
 from .truncation import ALICE, BOB
 
+_INT64 = torch.int64
+_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
 
 
@@ -67,32 +69,33 @@ class Rotary:
         self._dev = phases.get_device()
         self._pairs = (phases.data_ptr(), 2 * phases.numel(), self.interleaved, self.amplitude, self.frac_bits, self.ring_bw)
 
-    def _check(self, x):
-        if x.dtype is not torch.int64 or x.dim() != 3 or x.get_device() != self._dev:
+    def _strides(self, x):
+        if x.dtype is not _INT64 or x.dim() != 3 or x.get_device() != self._dev:
             raise L.MMHError(7, "Rotary: expected a 3-D int64 tensor [tokens, heads, head_dim] on the phases' device")
         if x.shape[2] != self.head_dim:
             raise L.MMHError(3, "Rotary: head_dim")
-        if x.stride(2) != 1 and self.head_dim != 1 and x.numel():
+        token, head, word = x.stride()
+        if word != 1 and self.head_dim != 1 and x.numel():
             raise L.MMHError(7, "Rotary: the words of a head must be contiguous")
+        return token, head
 
     def _args(self, x, positions):
-        self._check(x)
-        if positions.dtype is not torch.int64 or positions.dim() != 1 or positions.get_device() != self._dev or \
+        token, head = self._strides(x)
+        if positions.dtype is not _INT64 or positions.dim() != 1 or positions.get_device() != self._dev or \
                 not positions.is_contiguous():
             raise L.MMHError(7, "Rotary: expected contiguous int64 positions on the phases' device")
         tokens, heads, dim = x.shape
         if positions.shape[0] != tokens:
             raise L.MMHError(3, "Rotary: #positions")
-        st, sh, _ = x.stride()
-        return (x.data_ptr(), st, sh, tokens, heads, dim, positions.data_ptr(), *self._pairs)
+        return (x.data_ptr(), token, head, tokens, heads, dim, positions.data_ptr()) + self._pairs
 
-    def _call(self, fn, *args):
-        stream = torch._C._cuda_getCurrentRawStream(self._dev)
-        if torch.cuda.current_device() == self._dev:
-            rc = fn(*args, stream)
+    def _call(self, fn, args):
+        args += (_stream_of(self._dev),)
+        if _current_device() == self._dev:
+            rc = fn(*args)
         else:
             with torch.cuda.device(self._dev):
-                rc = fn(*args, stream)
+                rc = fn(*args)
         if rc:
             L.check(rc)
 
@@ -100,12 +103,12 @@ class Rotary:
         """the turned share, scaled by 2^frac_bits; ``out`` may be x (same strides), or another tensor of the shape"""
         args = self._args(x, positions)
         if out is None:
-            out = torch.empty(x.shape, dtype=torch.int64, device=x.device)
+            out = x.new_empty(x.shape)
+            token, head = args[4] * args[5], args[5]
         else:
-            self._check(out)
+            token, head = self._strides(out)
             _need(out.shape == x.shape, 3, "Rotary: out")
-        st, sh, _ = out.stride()
-        self._call(self.lib.mmh_rotary, *args, out.data_ptr(), st, sh)
+        self._call(self.lib.mmh_rotary, args + (out.data_ptr(), token, head))
         return out
 
     def truncate_pre(self, party, x, positions, signed_arithmetic=True, apply_msb0_heuristic=True):
@@ -113,8 +116,8 @@ class Rotary:
         heuristic, which does not compare)"""
         _need(party in (ALICE, BOB), 7, "Rotary: party")
         args = self._args(x, positions)
-        adj = torch.empty(x.shape, dtype=torch.int64, device=x.device)
+        adj = x.new_empty(x.shape)
         cmp = None if apply_msb0_heuristic else torch.empty_like(adj)
-        self._call(self.lib.mmh_rotary_trunc_pre, party, *args, bool(signed_arithmetic), bool(apply_msb0_heuristic),
-                   adj.data_ptr(), 0 if cmp is None else cmp.data_ptr())
+        self._call(self.lib.mmh_rotary_trunc_pre, (party,) + args + (bool(signed_arithmetic), bool(apply_msb0_heuristic),
+                                                                     adj.data_ptr(), 0 if cmp is None else cmp.data_ptr()))
         return adj, cmp
