@@ -6,9 +6,13 @@
 // digit + 128, the exclusive or takes the 128 off again as a signed byte).  l bits need nx = ceil(l/8) digits of x (what
 // lies above is a multiple of 2^l), a weight as many as its size asks for, found when the weights are laid out.  The
 // product modulo 2^l is then sum over s < nx of 256^s * sum_{i+j=s} x_i w_j, every inner sum an exact i8 x i8 -> i32
-// matrix product (v_mfma_i32_32x32x32_i8, 1.6 times the rate of the 16x16x64 form), nx accumulators per output.  |x_i w_j| <= 2^14 and at most nw products share
-// an accumulator, so up to (2^17 - 1) / nw terms of k cannot overflow; longer k is added up in 64-bit pieces.
-// Everything is exact: the result does not depend on the order of the sums.
+// matrix product, nx accumulators per output.  |x_i w_j| <= 2^14 and at most nw products share an accumulator, so up to
+// (2^17 - 1) / nw terms of k cannot overflow; longer k is added up in 64-bit pieces.  Everything is exact: the result does
+// not depend on the order of the sums.
+//
+// Bounds.  nx nw - nw (nw - 1) / 2 byte products per multiplication (15 for 64 bits and two-byte weights), at the rate
+// v_mfma_i32_32x32x32_i8 sustains on random digits from registers: 21 ns per instruction and SIMD, 3.2 P operations/s (4.2 P on
+// constant ones: the chip lowers its clock; the 16x16x64 form reaches 0.6 of that).  Few rows: the bytes of the weights' digits.
 #include <algorithm>
 #include <new>
 
@@ -135,17 +139,16 @@ __device__ __forceinline__ long long ring_token(const RingArgs &a, size_t r) {
   return t >= 0 && t < (long long)a.n_tokens ? t : -1;
 }
 
-// rows that no group has, in the columns [n0, n1): zeros, where the caller asked for them
-__device__ __forceinline__ void ring_zero_rest(const RingArgs &a, int n0, int n1) {
+// rows that no group has, in the columns [n0, n1): zeros, where the caller asked for them; workgroup `part` of `parts` on them
+__device__ __forceinline__ void ring_zero_rest(const RingArgs &a, int n0, int n1, u32 part, u32 parts) {
   if (!a.zero_rest || !a.offsets) return;
   const long long n = (long long)a.n_rows;
   long long b = a.offsets[0], e = a.offsets[a.groups];
   b = b < 0 ? 0 : b > n ? n : b, e = e < b ? b : e > n ? n : e;
   n1 = n1 < a.n_out ? n1 : a.n_out;
-  for (long long row = 0; row < n; ++row) {
-    if (row == b) row = e;
-    if (row >= n) break;
-    for (int i = n0 + (int)threadIdx.x; i < n1; i += blockDim.x) a.out[(size_t)row * a.ldo + i] = 0;
+  for (long long i = part; i < n - (e - b); i += parts) {
+    u64 *p = a.out + (size_t)(i < b ? i : i + (e - b)) * a.ldo;
+    for (int c = n0 + (int)threadIdx.x; c < n1; c += blockDim.x) p[c] = 0;
   }
 }
 
@@ -209,7 +212,7 @@ __device__ __forceinline__ int ring_piece(int cols, int place) { return cols < 6
 
 // Fewer than 4 columns: 64-bit products, one output a lane.
 __global__ __launch_bounds__(256) void ring_narrow_kernel(RingArgs a, int nw) {
-  if (blockIdx.y == 0) ring_zero_rest(a, (int)blockIdx.x * 256, (int)blockIdx.x * 256 + 256);
+  ring_zero_rest(a, (int)blockIdx.x * 256, (int)blockIdx.x * 256 + 256, blockIdx.y, gridDim.y);
   RingGroups<32> groups;
   RingTile tile;
   if (a.offsets) groups.load(a, 0);
@@ -235,13 +238,16 @@ __global__ __launch_bounds__(256) void ring_narrow_kernel(RingArgs a, int nw) {
 // through LDS.  Bound by latency: everything a wave needs of its first steps is asked for at once (kAhead steps), and it cuts
 // its own digits into LDS of its own, so the loop has no barrier.  16 x 16 products (v_mfma_i32_16x16x64_i8), of whose rows 8
 // stay zero: their rate does not matter here, their few registers do.  4 columns or more.
+// us by rows, 64 bits and two-byte weights, against the tile kernel with k split and its second launch:
+//   2048 -> 1001: 1 row 5.0 (11.3), 4 5.6 (11.5), 8 7.4 (11.5);  4096 -> 4096: 1 row 7.2 (15.0; 33.5 MB of digits = 4.7 TB/s),
+//   8 12.5 (15.7);  8192 -> 1024: 1 row 9.0 (19.1), 8 19.3 (18.9).  16 rows would read twice the words per workgroup.
 template <int NX, int NW, bool TWO>
 __global__ __launch_bounds__(1024) void ring_few_kernel(RingArgs a) {
   constexpr int W = 16, kAhead = NW <= 2 && !TWO ? 2 : 1;
   __shared__ uint4 lds[W][NX * 64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int ot = (int)blockIdx.x;   // 16 outputs
-  if (blockIdx.y == 0) ring_zero_rest(a, ot * 16, ot * 16 + 16);
+  ring_zero_rest(a, ot * 16, ot * 16 + 16, blockIdx.y, gridDim.y);
   RingGroups<8> groups;
   RingTile tile;
   if (a.offsets) groups.load(a, 0);
@@ -344,8 +350,10 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
   RingGroups<32> groups;
   if (a.offsets) groups.load(a, 0);
   const RingOrder order(a, ring_count_tiles(a, groups));
-  if (!a.ws)
-    for (int t = (int)blockIdx.x; t < a.out_tiles; t += gridDim.x) ring_zero_rest(a, t * 256 * OT, (t + 1) * 256 * OT);
+  if (!a.ws) {   // the grid has a workgroup for each output tile, at least
+    const u32 parts = gridDim.x / a.out_tiles, part = blockIdx.x / a.out_tiles, t = blockIdx.x - part * a.out_tiles;
+    if (part < parts) ring_zero_rest(a, t * 256 * OT, (t + 1) * 256 * OT, part, parts);
+  }
   const int last = a.k32 / 2 - 1;
   const int first = (int)((long long)(last + 1) * blockIdx.y / gridDim.y);
   const int end = (int)((long long)(last + 1) * (blockIdx.y + 1) / gridDim.y);
@@ -583,7 +591,8 @@ static void ring_launch_layout(const void *w, const mmh_ring_weights *h, hipStre
                      h->rows, h->cols, h->bw, h->out32, h->k32, h->nw, units, h->d);
 }
 
-// Parts of k for `tiles` workgroups of the tile kernel on the chip's 256 compute units, by a model of its time (us): rounds of
+// Parts of k, by which few tiles fill the chip (48 x 4096 x 4096 72 -> 29 us, 200 x 4096 x 1024 72 -> 26, 700 x 2048 x 1500 47 -> 44):
+// for `tiles` workgroups of the tile kernel on the chip's 256 compute units, by a model of its time (us): rounds of
 // workgroups, each with its steps and a start and end of its own, and the launch that adds up the parts, 16 bytes of traffic
 // per part and output.  A step of 30 products takes 1.45 us with all units busy, one of a few products no less than 1.
 static int ring_parts(size_t tiles, size_t steps, int products, size_t outputs) {

@@ -39,6 +39,8 @@ def test_rotary_refusals_without_gpu():
     assert call(x=None) == 2 and call(out=None) == 2 and call(pos=None) == 2 and call(ph=None) == 2
     assert call(rot=15) == 3 and call(rot=18) == 3 and call(d=0, rot=0) == 3
     assert call(oh=15) == 3 and call(ot=15) == 3  # rows of the result would overlap
+    assert call(oh=16, ot=63) == 3 and call(oh=31, ot=16) == 3 and call(oh=0, ot=0) == 3 and call(oh=0, ot=64) == 3
+    assert call(t=1, oh=15) == 3 and call(h=1, ot=15) == 3 and call(h=1, ot=0) == 3
     assert call(frac=25) == 7 and call(frac=-1) == 7 and call(bw=1) == 7 and call(bw=65) == 7
     assert call(amp=0.0) == 7 and call(amp=17.0) == 7 and call(amp=float("nan")) == 7 and call(amp=-1.0) == 7
     assert call(d=4097) == 6 and call(h=65537) == 6 and call(t=1 << 31) == 6
