@@ -8,8 +8,9 @@ clear and the server, which holds x1, computes its share
 
     y1 = W (x0 - r + x1) + s  mod 2^l        (``RingFCSS.matMul``: x = x0 - r, share1 = x1, add = s)
 
-so that y0 + y1 = W (x0 + x1).  Rows of several experts (adapters, clients' models) go through one call; which row belongs
-to which expert is public.  Same ``gemini::Code`` errors as the other layer classes.
+so that y0 + y1 = W (x0 + x1).  ``PreparedFCSS`` is that layer for both parties; rows of several experts (adapters, clients'
+models) go through one call, and which row belongs to which expert is public.  Same ``gemini::Code`` errors as the other layer
+classes.
 """
 import ctypes as C
 
@@ -153,3 +154,90 @@ class RingFCSS:
         if rc:
             L.check(rc)
         return out
+
+
+class PreparedFCSS:
+    """An FC layer of n rows over one or more weight matrices whose ciphertext work precedes the input.  BOB:
+
+        cts = bob.prepareMasks(n, meta)          -> ALICE   (one Enc(r) per row)
+        bob.finishMasks(out_cts)                 <- ALICE   (out_cts of prepareRows)
+        opened, y0 = bob.openInput(x0)           -> ALICE   (x0 - r; y0 is BOB's share of the result)
+
+    ALICE:  prepareWeights(w) once, out_cts = prepareRows(cts, offsets), y1 = online(opened, x1).
+
+    Rows offsets[g] .. offsets[g + 1] use matrix g.  A mask serves one input: a second openInput, or online, needs new masks.
+    ``exact`` keeps the noise terms the approximate re-sharing of ``HomFCSS.matVecMul`` leaves out (shares then add up exactly,
+    otherwise within 1)."""
+
+    def __init__(self):
+        from .hom_fc_ss import HomFCSS
+        self.fc, self.ring = HomFCSS(), RingFCSS()
+        self.sampler = self.weights = self._masks = self._y0 = self._s = None
+
+    def setUp(self, ctx, sampler, sk_ntt=None, pk_ntt=None, exact=False):
+        _need(ctx.t >= 4 and ctx.t & (ctx.t - 1) == 0, 1, "setUp: the plain modulus is not a ring 2^l")
+        self.ctx, self.sampler, self.exact = ctx, sampler, exact
+        self.fc.setUp(ctx, sk_ntt=sk_ntt, pk_ntt=pk_ntt)
+        self.ring.setUp(ctx.t.bit_length() - 1)
+        return 0
+
+    # -- BOB
+    def prepareMasks(self, n, meta):
+        _need(self.sampler is not None, 1, "prepareMasks: setUp first")
+        cols, p = meta.input_shape[0], self.fc.plan(meta)
+        r = (self.sampler.words(n * cols) & (self.ctx.t - 1)).view(n, cols)
+        cts = [self.fc.encryptInputVector(v, meta, (self.sampler.uniform(p.n_in), self.sampler.noise(p.n_in))) for v in r]
+        self._masks, self._y0, self._meta = r, None, meta
+        return cts
+
+    def finishMasks(self, out_cts):
+        _need(self._masks is not None and len(out_cts) == self._masks.shape[0], 3, "finishMasks: #rows")
+        y0 = self._masks.new_empty((len(out_cts), self._meta.weight_shape[0]))
+        for row, ct in zip(y0, out_cts):
+            row.copy_(self.fc.decryptToVector(ct, self._meta))
+        self._y0 = y0
+
+    def openInput(self, x0):
+        _need(self._y0 is not None, 1, "openInput: no masks that were not used")
+        _need(tuple(x0.shape) == tuple(self._masks.shape), 3, "openInput: input shape")
+        opened, y0 = (x0 - self._masks) & (self.ctx.t - 1), self._y0
+        self._masks = self._y0 = None
+        return opened, y0
+
+    # -- ALICE
+    def prepareWeights(self, w, meta):
+        """w [groups, rows, cols], int64 ring elements (values below 2^l or signed)"""
+        _need(self.sampler is not None, 1, "prepareWeights: setUp first")
+        _need(w.dim() == 3 and tuple(w.shape[1:]) == tuple(meta.weight_shape), 3, "prepareWeights: weight shape")
+        self.weights, self._meta = self.ring.encodeWeights(w), meta
+        self._plain = [self.fc.encodeWeightMatrix(m, meta) for m in (w & (self.ctx.t - 1)).contiguous()]
+
+    def prepareRows(self, cts, offsets):
+        """the ciphertexts of W_g r - s for BOB; offsets: groups + 1 integers on the host, every row in a group"""
+        offsets = [int(v) for v in offsets]
+        _need(self.weights is not None, 1, "prepareRows: prepareWeights first")
+        _need(len(offsets) == self.weights.groups + 1 and offsets[0] == 0 and offsets[-1] == len(cts) and
+              all(a <= b for a, b in zip(offsets, offsets[1:])), 3, "prepareRows: offsets")
+        from .hom_fc_ss import Meta
+        meta = Meta(self._meta.weight_shape, self._meta.input_shape, False)    # the mask is BOB's alone
+        n, N, smp, out, s = self.fc.plan(meta).n_out, self.ctx.N, self.sampler, [], []
+        for g, plain in enumerate(self._plain):
+            for ct in cts[offsets[g]:offsets[g + 1]]:
+                if self.exact:
+                    rand = (smp.words(n * N).view(n, N), smp.ternary(n), smp.noise(n), smp.noise(n), smp.words(n * N).view(n, N))
+                else:
+                    rand = smp.reshare(n)
+                c, share = self.fc.matVecMul(plain, ct, None, meta, rand, exact=self.exact)
+                out.append(c)
+                s.append(share)
+        dev = self.weights.device
+        self._s = torch.stack(s) if s else torch.empty((0, self.weights.rows), dtype=_INT64, device=f"cuda:{dev}")
+        self._offsets = torch.tensor(offsets, dtype=_INT64, device=f"cuda:{dev}")
+        return out
+
+    def online(self, opened, share1):
+        _need(self._s is not None, 1, "online: no rows prepared that were not used")
+        _need(opened.shape[0] == self._s.shape[0], 3, "online: #rows")
+        y1 = self.ring.matMul(self.weights, opened, self._offsets, share1=share1, add=self._s, out=self._s)
+        self._s = None
+        return y1

@@ -221,54 +221,44 @@ def _two_parties(run):
 
 def test_two_party_projection_turn_truncation(mm):
     """A query projection in two adapters' weights, the turn and one truncation, between two parties: the ciphertext product of
-    the client's masks runs ahead (HomFCSS), the online product on opened inputs (RingFCSS), then Truncation.truncate_rotary.
+    the client's masks runs ahead and the online product takes opened inputs (PreparedFCSS), then Truncation.truncate_rotary.
     The shares add up to the turned projection within the one unit the truncation gives up, plus the unit of its floor."""
-    import torch
-    from openmm_amd.hom_fc_ss import HomFCSS, Meta
-    from openmm_amd.lib import Sampler
-    from openmm_amd.ring_fc_ss import RingFCSS
+    from openmm_amd.hom_fc_ss import Meta
+    from openmm_amd.lib import MMHError, Sampler
+    from openmm_amd.ring_fc_ss import PreparedFCSS
     from openmm_amd.rotary import Rotary, rotary_phases
-    from openmm_amd.truncation import ALICE, IdealAux, Truncation
+    from openmm_amd.truncation import IdealAux, Truncation
     bw, scale, frac = 44, 8, 10
     tokens, cols, heads, dim = 9, 48, 2, 16
     rows, groups = heads * dim, 2
     off, ring = np.array([0, 4, 9]), 1 << bw
     r = np.random.default_rng(SEED)
     xs = r.integers(-1 << scale, 1 << scale, (tokens, cols))                # values in (-1, 1)
-    w = r.integers(-1 << scale, 1 << scale, (groups, rows, cols)).astype(np.int16)
+    w = r.integers(-1 << scale, 1 << scale, (groups, rows, cols))
+    w[w == 0] = 1                                                           # HomFCSS refuses blocks of zeros
     pos = r.integers(0, 100000, tokens)
     x0 = words(SEED, (tokens, cols), bw)
     x1 = (xs.astype(np.int64).view(np.uint64) - x0) & mask(bw)
-    # ahead of the input: Enc(r) -> Enc(W r - s), a row at a time; BOB keeps W r - s, ALICE keeps s
     ctx = mm.Context(4096, (60, 49), ring)
     smp = Sampler(ctx, key=bytes(range(32)))
     sk, pk = smp.keygen()
-    client, server = HomFCSS(), HomFCSS()
-    client.setUp(ctx, sk_ntt=sk, pk_ntt=pk)
-    server.setUp(ctx, pk_ntt=pk)
-    meta = Meta((rows, cols), (cols,), False)
-    wr = w.astype(np.int64).view(np.uint64) & mask(bw)
-    wr[wr == 0] = 1
-    w = wr.view(np.int64)                 # a weight of zero became one: HomFCSS refuses blocks of zeros
-    rnd = words(SEED + 9, (tokens, cols), bw)
-    y0, s = [], []
-    for t in range(tokens):
-        g = int(np.searchsorted(off, t, "right")) - 1
-        plan = client.plan(meta)
-        cts = client.encryptInputVector(dev(rnd[t]), meta, (smp.uniform(plan.n_in), smp.noise(plan.n_in)))
-        n = plan.n_out
-        rand = (smp.words(n * ctx.N).view(n, -1), smp.ternary(n), smp.noise(n), smp.noise(n), smp.words(n * ctx.N).view(n, -1))
-        out, share = server.matVecMul(server.encodeWeightMatrix(dev(wr[g]), meta), cts, None, meta, rand, exact=True)
-        y0.append(client.decryptToVector(out, meta))
-        s.append(share)
-    y0, s = torch.stack(y0), torch.stack(s)
-    # online
-    f = RingFCSS()
-    f.setUp(bw)
-    opened = dev((x0 - rnd) & mask(bw))
-    y1 = f.matMul(f.encodeWeights(dev(w)), opened, dev(off), share1=dev(x1), add=s)
+    meta = Meta((rows, cols), (cols,), True)
     want = product(xs.astype(np.int64).view(np.uint64), w, bw, off)
-    assert np.array_equal((host(y0) + host(y1)) & mask(bw), want)
+    signed = lambda v: ((v.astype(object) + ring // 2) % ring - ring // 2)
+    for exact in (False, True):
+        bob, alice = PreparedFCSS(), PreparedFCSS()
+        bob.setUp(ctx, smp, sk_ntt=sk)
+        alice.setUp(ctx, smp, pk_ntt=pk, exact=exact)
+        alice.prepareWeights(dev(w), meta)
+        bob.finishMasks(alice.prepareRows(bob.prepareMasks(tokens, meta), off))
+        opened, y0 = bob.openInput(dev(x0))
+        y1 = alice.online(opened, dev(x1))
+        err = signed((host(y0) + host(y1) - want) & mask(bw)).astype(np.int64)
+        assert np.abs(err).max() <= (0 if exact else 1)
+        for again in (lambda: bob.openInput(dev(x0)), lambda: alice.online(opened, dev(x1))):   # masks serve once
+            with pytest.raises(MMHError) as e:
+                again()
+            assert e.value.code == 1
     # each party turns and truncates its own share: one truncation takes off the product's and the turn's scale
     ph, aux = rotary_phases(dim), IdealAux()
     share = {1: y1, 2: y0}
@@ -280,7 +270,6 @@ def test_two_party_projection_turn_truncation(mm):
     got = _two_parties(party)
     total = (host(got[1]) + host(got[2])) & mask(bw)
     turned = rotary(want.reshape(tokens, heads, dim), pos, ph, frac, bw)
-    signed = lambda v: ((v.astype(object) + ring // 2) % ring - ring // 2)
     exact = signed(turned) // (1 << (scale + frac))
     assert np.abs((signed(total) - exact).astype(np.int64)).max() <= 1
     # and without the heuristic, through the comparison
