@@ -110,28 +110,21 @@ __device__ __forceinline__ u32 ring_count_tiles(const RingArgs &a, const RingGro
   return n;
 }
 
-// The tiles of a workgroup.  Workgroups go round the 8 XCDs, each with an L2 of its own; what runs on an XCD at one time should
-// share rows and weights.  Its tiles are taken in the order "16 output tiles across, row tiles down", one workgroup the next to
-// its neighbour's: with eight row tiles or more an XCD has every eighth of them, else a contiguous piece of that order.  (Four
-// across reads rows four times over where they come from memory: 8192 x 4096 x 4096 with two shares 1.97 ms against 1.91.)
-struct RingOrder {
-  static constexpr u32 kAcross = 16;
-  u32 rows, out_tiles, base, count;   // row tiles in the order, tiles before and in this XCD's piece
-  bool deal;
-  __device__ __forceinline__ RingOrder(const RingArgs &a, u32 row_tiles) : out_tiles((u32)a.out_tiles), deal(row_tiles >= 8) {
-    const u32 xcd = blockIdx.x & 7;
-    rows = deal ? (row_tiles - xcd + 7) / 8 : row_tiles;
-    const u32 total = out_tiles * rows, per = (total + 7) / 8;
-    base = deal ? 0 : xcd * per;
-    count = deal ? total : base >= total ? 0 : total - base < per ? total - base : per;
-  }
-  __device__ __forceinline__ void tile(u32 i, int &ot, u32 &rt) const {
-    const u32 q = base + i, panel = q / (kAcross * rows), rest = q - panel * kAcross * rows;
-    const u32 wide = out_tiles - panel * kAcross < kAcross ? out_tiles - panel * kAcross : kAcross;
-    rt = rest / wide, ot = (int)(panel * kAcross + rest % wide);
-    if (deal) rt = rt * 8 + (blockIdx.x & 7);
-  }
-};
+// The tile of a workgroup.  Workgroups go round the 8 XCDs, each with an L2 of its own; what runs on an XCD at one time should
+// share rows and weights, so each has a contiguous piece of the order "16 output tiles across, row tiles down", of the row tiles
+// that the groups have.  (Four across reads rows four times over where they come from memory: 8192 x 4096 x 4096 with two shares
+// 1.97 ms against 1.91.  Row tiles dealt out to the XCDs one by one leave up to a row of tiles more on one of them: 777 x 1023 x 515
+// in three parts 30 us.)
+__device__ __forceinline__ bool ring_block(const RingArgs &a, u32 row_tiles, int &ot, u32 &rt) {
+  constexpr u32 kAcross = 16;
+  const u32 out_tiles = (u32)a.out_tiles, total = out_tiles * row_tiles, per = (total + 7) / 8;
+  const u32 q = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || q >= total) return false;
+  const u32 panel = q / (kAcross * row_tiles), rest = q - panel * kAcross * row_tiles;
+  const u32 wide = out_tiles - panel * kAcross < kAcross ? out_tiles - panel * kAcross : kAcross;
+  rt = rest / wide, ot = (int)(panel * kAcross + rest % wide);
+  return true;
+}
 
 // the row of x that row r reads, or -1 (an index outside [0, n_tokens) reads as a row of zeros)
 __device__ __forceinline__ long long ring_token(const RingArgs &a, size_t r) {
@@ -349,7 +342,6 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
   const int r = lane & 15, sub = lane >> 4;
   RingGroups<32> groups;
   if (a.offsets) groups.load(a, 0);
-  const RingOrder order(a, ring_count_tiles(a, groups));
   if (!a.ws) {   // the grid has a workgroup for each output tile, at least
     const u32 parts = gridDim.x / a.out_tiles, part = blockIdx.x / a.out_tiles, t = blockIdx.x - part * a.out_tiles;
     if (part < parts) ring_zero_rest(a, t * 256 * OT, (t + 1) * 256 * OT, part, parts);
@@ -360,8 +352,7 @@ __global__ __launch_bounds__(512, 2) void ring_tile_kernel(RingArgs a) {
 
   u32 rt;
   RingTile tile;
-  if (blockIdx.x >> 3 >= order.count) return;
-  order.tile(blockIdx.x >> 3, tile.ot, rt);
+  if (!ring_block(a, ring_count_tiles(a, groups), tile.ot, rt)) return;
   if (!ring_find_tile(a, groups, rt, tile)) return;
   const size_t lo = tile.lo, hi = tile.hi;
   const int ot0 = (tile.ot * 8 + wave) * OT;
@@ -591,19 +582,20 @@ static void ring_launch_layout(const void *w, const mmh_ring_weights *h, hipStre
                      h->rows, h->cols, h->bw, h->out32, h->k32, h->nw, units, h->d);
 }
 
-// Parts of k, by which few tiles fill the chip (48 x 4096 x 4096 72 -> 29 us, 200 x 4096 x 1024 72 -> 26, 700 x 2048 x 1500 47 -> 44):
-// for `tiles` workgroups of the tile kernel on the chip's 256 compute units, by a model of its time (us): rounds of
-// workgroups, each with its steps and a start and end of its own, and the launch that adds up the parts, 16 bytes of traffic
-// per part and output.  A step of 30 products takes 1.45 us with all units busy, one of a few products no less than 1.
+// Parts of k, by which few tiles fill the chip (48 x 4096 x 4096 72 -> 28 us, 200 x 4096 x 1024 72 -> 26, 64 x 1024 x 1024 23 -> 13),
+// by a model of the tile kernel's time (us): rounds of workgroups on the 32 compute units of each XCD, each round its steps and 5
+// us for its start and its results; the second launch and 16 bytes of traffic per part and output.  A step of 30 products takes
+// 1.05 us on a few compute units and 1.45 with all of them busy, one of a few products no less than 0.9.
 static int ring_parts(size_t tiles, size_t steps, int products, size_t outputs) {
-  const double step = std::max(1.0, products * (1.45 / 30));
+  auto time = [&](int p) {
+    const double busy = std::min(1.0, (double)(tiles * p) / 256), step = std::max(0.9, products * (0.035 + 0.0133 * busy));
+    const double rounds = (double)(((tiles + 7) / 8 * p + 31) / 32);
+    return rounds * ((double)((steps + p - 1) / p) * step + 5) + (p > 1 ? 2.5 + p * (double)outputs * 16 / 2.8e6 : 0);
+  };
   int best = 1;
-  double least = 0;
-  for (int p = 1; p <= 16 && (size_t)p * 2 <= std::max<size_t>(steps, 2); ++p) {
-    const double rounds = (double)((tiles * p + 255) / 256);
-    const double t = rounds * ((double)((steps + p - 1) / p) * step + 5) + (p > 1 ? 5 + p * (double)outputs * 16 / 4.5e6 : 0);
-    if (p == 1 || t < 0.9 * least) best = p, least = t;
-  }
+  double least = 0.9 * time(1);   // one launch unless two are clearly faster
+  for (int p = 2; p <= 16 && (size_t)p * 2 <= steps; ++p)
+    if (time(p) < least) best = p, least = time(p);
   return best;
 }
 // up to 8 rows in all go to ring_few_kernel, whose waves must not sum more columns than fit 32 bits
@@ -627,7 +619,7 @@ static int ring_call_parts(int nx, int nw, bool two, size_t out32, size_t row_ti
 template <int NX, int NW, int OT, bool TWO>
 static void ring_launch_tiles(RingArgs a, hipStream_t s, int parts) {
   a.out_tiles = (int)ring_out_tiles(a.out32, OT);
-  const dim3 grid((a.row_tiles >= 8 ? (a.row_tiles + 7) / 8 * a.out_tiles : (a.row_tiles * a.out_tiles + 7) / 8) * 8, parts);
+  const dim3 grid((a.row_tiles * a.out_tiles + 7) / 8 * 8, parts);
   hipLaunchKernelGGL((ring_tile_kernel<NX, NW, OT, TWO>), grid, dim3(512), 0, s, a);
 }
 template <int NX, int NW, bool TWO>
