@@ -723,14 +723,15 @@ int mmh_ring_weights_create(const void *d_w, int elem_bytes, size_t n_groups, si
                             void *stream, mmh_ring_weights **out);
 int mmh_ring_weights_destroy(mmh_ring_weights *w);
 int mmh_ring_weights_info(const mmh_ring_weights *w, size_t *n_groups, size_t *rows, size_t *cols, int *ring_bw, int *digits);
-/* d_x [n_tokens] rows of cols words, ldx words apart; d_x1 (may be NULL) the same shape, ldx1 apart; any 64-bit words,
- * taken mod 2^ring_bw.  d_rows [n_rows] (NULL: row r reads token r) may name a token any number of times; an index outside
- * [0, n_tokens) reads as a row of zeros.  d_offsets [n_groups + 1], non-decreasing (NULL with one group: all rows); values
- * are clamped to [0, n_rows] and output rows outside every group are left as they were, or set to zero with zero_rest.  d_add (may be NULL) n_rows rows
- * ldadd apart (0: one row for all); it may be d_out with ldadd = ldo.  d_out must not overlap the other inputs.  Results
- * are reduced mod 2^ring_bw and exact.  d_ws (may be NULL) is scratch of ws_words words for this call alone: with the
- * mmh_ring_matmul_workspace words small calls are faster, with fewer (or none) they run without it.  The call allocates
- * nothing and may be captured; calls on different streams touch nothing in common.  Runs on the weights' device.  n_rows <= 2^19 per call, n_groups <= 32767. */
+/* d_x [n_tokens] rows of cols words, ldx words apart (0: one row for all); d_x1 (may be NULL) the same shape, ldx1 apart; any
+ * 64-bit words, taken mod 2^ring_bw.  d_rows [n_rows] (NULL: row r reads token r) may name a token any number of times; an
+ * index outside [0, n_tokens) reads as a row of zeros.  d_offsets [n_groups + 1], non-decreasing (NULL with one group: all
+ * rows); values are clamped to [0, n_rows], and output rows outside every group are left as they were, or set to zero with
+ * zero_rest.  d_add (may be NULL) n_rows rows ldadd apart (0: one row for all); it may be d_out with ldadd = ldo.  d_out must
+ * not overlap the other inputs.  Results are reduced mod 2^ring_bw and exact.
+ * d_ws (may be NULL) is scratch of ws_words words for this call alone: with the mmh_ring_matmul_workspace words small calls are
+ * faster, with fewer (or none) they run without it.  The call allocates nothing and may be captured; calls on different streams
+ * touch nothing in common.  Runs on the weights' device.  n_rows <= 2^19 per call, n_groups <= 32767. */
 int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, size_t ldx, const uint64_t *d_x1, size_t ldx1,
                     size_t n_tokens, const int64_t *d_rows, const int64_t *d_offsets, size_t n_rows, const uint64_t *d_add,
                     size_t ldadd, uint64_t *d_out, size_t ldo, int zero_rest, uint64_t *d_ws, size_t ws_words, void *stream);

@@ -773,7 +773,8 @@ extern "C" int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, s
   MMH_REQUIRE(d_out && d_x, MMH_ERR_NULL_POINTER);
   MMH_REQUIRE(d_offsets || w->groups == 1, MMH_ERR_NULL_POINTER);
   MMH_REQUIRE(n_tokens >= 1 && (d_rows || n_rows <= n_tokens), MMH_ERR_DIM_MISMATCH);
-  MMH_REQUIRE(ldx >= w->cols && (!d_x1 || ldx1 >= w->cols) && ldo >= w->rows, MMH_ERR_DIM_MISMATCH);
+  MMH_REQUIRE((ldx == 0 || ldx >= w->cols) && (!d_x1 || ldx1 == 0 || ldx1 >= w->cols), MMH_ERR_DIM_MISMATCH);
+  MMH_REQUIRE(ldo >= w->rows, MMH_ERR_DIM_MISMATCH);
   MMH_REQUIRE(!d_add || ldadd == 0 || ldadd >= w->rows, MMH_ERR_DIM_MISMATCH);
   // row tiles are the second dimension of a grid, which the hardware counts in 16 bits, and with the output tiles the first
   MMH_REQUIRE(n_rows <= (size_t(1) << 19) && w->groups <= 32767, MMH_ERR_OUT_BOUND);

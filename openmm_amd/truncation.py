@@ -242,6 +242,8 @@ class Truncation:
         # what mmh_trunc_post asks for, before the protocol starts
         if not (1 <= shift < bw and (not apply_msb0_heuristic or shift <= bw - 3)):
             raise L.MMHError(7, "truncate_rotary: shift")
+        if x.get_device() != self.device:
+            raise L.MMHError(7, "truncate_rotary: x on another device than the protocol's")
         adj, cmp = rotary.truncate_pre(self.party, x, positions, signed_arithmetic, apply_msb0_heuristic)
         if dim == 0:
             return adj

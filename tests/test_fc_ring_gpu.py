@@ -179,6 +179,11 @@ def test_strides(mm, tokens, pad, shift):
     assert np.array_equal(host(out.contiguous()), product(x, w, bw, None, None, x1, add))
     out.fill_(77)
     assert bool((buf == 77).all())      # nothing written between the rows
+    # one row for all of them
+    y = f.matMul(rw, dev(x[:1]).expand(tokens, cols), share1=dev(x1), add=dev(add[:1]).expand(tokens, rows))
+    assert np.array_equal(host(y), product(np.repeat(x[:1], tokens, 0), w, bw, None, None, x1, add[0]))
+    y = f.matMul(rw, dev(x), share1=dev(x1[:1]).expand(tokens, cols))
+    assert np.array_equal(host(y), product(x, w, bw, None, None, np.repeat(x1[:1], tokens, 0)))
 
 
 # k over several workgroups, whose sums a second launch joins (a few rows against long columns), and the same without scratch
