@@ -17,7 +17,6 @@
 #include <new>
 
 #include "common.hpp"
-#include "convert_device.hpp"
 
 struct mmh_ring_weights {
   int device = 0;
@@ -107,7 +106,7 @@ __device__ __forceinline__ u32 ring_count_tiles(const RingArgs &a, const RingGro
     more.load(a, g0);
     n += more.total();
   }
-  return n;
+  return n < (u32)a.row_tiles ? n : (u32)a.row_tiles;   // groups that overlap, which none may, could have more than the grid
 }
 
 // The tile of a workgroup.  Workgroups go round the 8 XCDs, each with an L2 of its own; what runs on an XCD at one time should

@@ -156,6 +156,22 @@ def test_padding_and_bad_indices(mm, scale):
     assert np.array_equal(host(f.matMul(rw, dev(x), dev(under))), product(x, w, bw, off))
 
 
+# offsets that no caller may pass (decreasing, overlapping, far outside): whatever comes out, nothing but the result is written
+@pytest.mark.parametrize("cols,n", [(1, 70), (40, 6), (130, 70), (2048, 70)])
+def test_offsets_out_of_order(mm, cols, n):
+    import torch
+    g, rows = 100, 37
+    f = fc(64)
+    rw = f.encodeWeights(dev(weights(SEED, (g, rows, cols), np.int16)))
+    x = dev(words(SEED, (n, cols)))
+    r = np.random.default_rng(SEED)
+    for off in (r.integers(-5, n + 5, g + 1), r.integers(-1 << 62, 1 << 62, g + 1), np.where(np.arange(g + 1) % 2, n, 0)):
+        buf = torch.full((n + 20, rows), 9, dtype=torch.int64, device="cuda")
+        f.matMul(rw, x, dev(off.astype(np.int64)), out=buf[10:10 + n])
+        f.matMul(rw, x, dev(off.astype(np.int64)))
+        assert bool((buf[:10] == 9).all()) and bool((buf[10 + n:] == 9).all())
+
+
 # strides and alignment: rows of wider arrays, odd strides, data at 8 modulo 16
 @pytest.mark.parametrize("tokens", [5, 50])
 @pytest.mark.parametrize("pad,shift", [(3, 0), (4, 1), (0, 1), (2, 0)])
@@ -246,10 +262,11 @@ def test_far_rows(mm):
     assert np.array_equal(host(out.contiguous()), product(x, w, bw))
 
 
-def test_streams_and_replays(mm):
-    """two calls at once on two streams; a captured call replayed among eager work"""
+@pytest.mark.parametrize("cols", [200, 2048])      # one launch, and two with scratch between them
+def test_streams_and_replays(mm, cols):
+    """two calls at once on two streams; captured calls replayed among eager work, each graph with scratch of its own"""
     import torch
-    cols, rows, bw = 200, 100, 64
+    rows, bw = 100, 64
     f = fc(bw)
     w = [weights(SEED + i, (2, rows, cols), np.int16) for i in range(2)]
     x = [words(SEED + i, (60, cols)) for i in range(2)]
@@ -266,17 +283,24 @@ def test_streams_and_replays(mm):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(np.array_equal(host(y), want[i]) for y in got[i])
-    out = torch.zeros((60, rows), dtype=torch.int64, device="cuda")
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        f.matMul(rw[0], dx[0], doff, out=out)
+    assert (rw[0].workspace(60) > 0) == (cols == 2048)
+    outs = [torch.zeros((60, rows), dtype=torch.int64, device="cuda") for _ in range(2)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for k in range(2):
+        with torch.cuda.graph(graphs[k]):
+            f.matMul(rw[k], dx[0], doff, out=outs[k])
+    expect = [[product(v, u, bw, off) for v in x] for u in w]
     for i in (0, 1, 0, 1):
         dx[0].copy_(dx[1] if i else dev(x[0]))
-        out.fill_(-1)
-        graph.replay()
+        for o in outs:
+            o.fill_(-1)
+        torch.cuda.synchronize()
+        for k, s in enumerate(streams):      # both graphs at once
+            with torch.cuda.stream(s):
+                graphs[k].replay()
         eager = f.matMul(rw[0], dx[0], doff)
         torch.cuda.synchronize()
-        assert np.array_equal(host(out), product(x[i], w[0], bw, off)) and torch.equal(out, eager)
+        assert all(np.array_equal(host(outs[k]), expect[k][i]) for k in range(2)) and torch.equal(outs[0], eager)
 
 
 def test_refusals(mm):
