@@ -592,7 +592,7 @@ static int ring_parts(size_t tiles, size_t steps, int products, size_t outputs) 
     return rounds * ((double)((steps + p - 1) / p) * step + 5) + (p > 1 ? 2.5 + p * (double)outputs * 16 / 2.8e6 : 0);
   };
   int best = 1;
-  double least = 0.9 * time(1);   // one launch unless two are clearly faster
+  double least = 0.95 * time(1);   // one launch unless two are faster
   for (int p = 2; p <= 16 && (size_t)p * 2 <= steps; ++p)
     if (time(p) < least) best = p, least = time(p);
   return best;
