@@ -44,13 +44,15 @@ class HomFCSS:
         self._plans = {}
 
     def setUp(self, ctx, sk_ntt=None, pk_ntt=None):  # hom_fc_ss.cc:129-155
+        if ctx is not self.ctx:
+            self._plans = {}   # a plan holds its context's degree and limbs
         self.ctx, self.sk_ntt, self.pk_ntt = ctx, sk_ntt, pk_ntt
         self.pk_last = None if pk_ntt is None else pk_ntt[:, :1].contiguous()
         self.sk_last = None if sk_ntt is None else sk_ntt[:1].contiguous()
         return 0
 
     def plan(self, meta):
-        key = (tuple(meta.weight_shape), bool(meta.is_shared_input))
+        key = (tuple(meta.weight_shape), tuple(meta.input_shape), bool(meta.is_shared_input))
         if key not in self._plans:
             self._plans[key] = Plan(self.ctx, meta)
         return self._plans[key]
