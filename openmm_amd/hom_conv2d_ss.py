@@ -112,6 +112,8 @@ class HomConv2DSS:
 
     # HomConv2DSS::setUp (hom_conv2d_ss.cc:467-495): sk_ntt [L,N] (client), pk_ntt [2,L,N] (server)
     def setUp(self, ctx, sk_ntt=None, pk_ntt=None):
+        if ctx is not self.ctx:
+            self._plans = {}   # a plan holds its context's degree and limbs
         self.ctx, self.sk_ntt, self.pk_ntt = ctx, sk_ntt, pk_ntt
         self.pk_last = None if pk_ntt is None else pk_ntt[:, :1].contiguous()
         self.sk_last = None if sk_ntt is None else sk_ntt[:1].contiguous()
