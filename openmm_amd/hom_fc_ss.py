@@ -62,10 +62,18 @@ class HomFCSS:
         if not cond:
             raise L.MMHError(code, what)
 
+    def _words(self, what, *tensors):
+        """the device reads 64-bit words through their pointers"""
+        for t in tensors:
+            self._need(t is None or t.element_size() == 8, 7, what + ": expected 64-bit words")
+
     def encryptInputVector(self, vec, meta, rand):  # :214-273
         self._need(self.ctx is not None and self.sk_ntt is not None, 1, "encryptInputVector: no secret key")
         self._need(tuple(vec.shape) == tuple(meta.input_shape), 3, "encryptInputVector: input shape")
         p, (a, e) = self.plan(meta), rand
+        self._need(a.numel() == p.n_in * self.ctx.L * self.ctx.N and e.numel() == p.n_in * self.ctx.N, 3,
+                   "encryptInputVector: rand shape")
+        self._words("encryptInputVector", vec, a, e)
         out = self.ctx._empty(p.n_in, 2, self.ctx.L, self.ctx.N)
         L.check(self.ctx.lib.mmh_fc_encrypt_input(p.handle, L.dptr(self.sk_ntt), L.dptr(vec), L.dptr(a), L.dptr(e),
                                                   L.dptr(out), L._stream_ptr()))
@@ -73,6 +81,7 @@ class HomFCSS:
 
     def encodeInputVector(self, vec, meta):  # :275-325
         self._need(tuple(vec.shape) == tuple(meta.input_shape), 3, "encodeInputVector: input shape")
+        self._words("encodeInputVector", vec)
         p = self.plan(meta)
         out = self.ctx._empty(p.n_in, self.ctx.N)
         L.check(self.ctx.lib.mmh_fc_encode_input(p.handle, L.dptr(vec), L.dptr(out), L._stream_ptr()))
@@ -80,6 +89,7 @@ class HomFCSS:
 
     def encodeWeightMatrix(self, w, meta):  # :327-392 -> [n_out, n_in, N]
         self._need(tuple(w.shape) == tuple(meta.weight_shape), 3, "encodeWeightMatrix: weight shape")
+        self._words("encodeWeightMatrix", w)
         p = self.plan(meta)
         out = self.ctx._empty(p.n_out, p.n_in, self.ctx.N)
         L.check(self.ctx.lib.mmh_fc_encode_weights(p.handle, L.dptr(w), L.dptr(out), L._stream_ptr()))
@@ -101,6 +111,7 @@ class HomFCSS:
             self._need(r is not None and tuple(r.shape) == (p.n_out, self.ctx.N), 3, "matVecMul: rand shape")
         self._need(tuple(matrix.shape) == (p.n_out, p.n_in, self.ctx.N), 7, "matVecMul: weight plaintexts shape")
         self._need(tuple(matrix.shape[:2]) == (p.n_out, p.n_in), 7, "matVecMul: #weight blocks")
+        self._words("matVecMul", matrix, vec_share0, vec_share1, *rand)
         # :414-422: a sub-matrix that encodes to zero is rejected
         nz = getattr(matrix, "_mm_nonzero", None)
         if nz is None:
@@ -128,7 +139,9 @@ class HomFCSS:
     def decryptToVector(self, enc_vector, meta):  # :572-602
         self._need(self.sk_ntt is not None, 1, "decryptToVector: no secret key")
         p = self.plan(meta)
-        self._need(enc_vector.shape[0] == p.n_out, 7, "decryptToVector: #ciphertexts")
+        self._need(enc_vector.shape[0] == p.n_out and enc_vector.numel() == p.n_out * 2 * self.ctx.N, 7,
+                   "decryptToVector: #ciphertexts")
+        self._words("decryptToVector", enc_vector)
         out = self.ctx._empty(meta.weight_shape[0])
         L.check(self.ctx.lib.mmh_fc_decrypt(p.handle, L.dptr(self.sk_last), L.dptr(enc_vector), L.dptr(out),
                                             L._stream_ptr()))
