@@ -166,16 +166,23 @@ class PreparedFCSS:
     ALICE:  prepareWeights(w) once, out_cts = prepareRows(cts, offsets), y1 = online(opened, x1).
 
     Rows offsets[g] .. offsets[g + 1] use matrix g.  A mask serves one input: a second openInput, or online, needs new masks.
+    setUp, new masks, new weights and new rows each drop what was prepared before them.
     ``exact`` keeps the noise terms the approximate re-sharing of ``HomFCSS.matVecMul`` leaves out (shares then add up exactly,
     otherwise within 1)."""
 
     def __init__(self):
         from .hom_fc_ss import HomFCSS
         self.fc, self.ring = HomFCSS(), RingFCSS()
-        self.sampler = self.weights = self._masks = self._y0 = self._s = None
+        self._forget()
+
+    def _forget(self):
+        self.sampler = self.weights = self._plain = self._masks = self._y0 = self._s = self._offsets = None
 
     def setUp(self, ctx, sampler, sk_ntt=None, pk_ntt=None, exact=False):
         _need(ctx.t >= 4 and ctx.t & (ctx.t - 1) == 0, 1, "setUp: the plain modulus is not a ring 2^l")
+        of = lambda c: (c.N, c.q, c.device)
+        _need(of(sampler.ctx) == of(ctx), 7, "setUp: the sampler draws for another context")
+        self._forget()
         self.ctx, self.sampler, self.exact = ctx, sampler, exact
         self.fc.setUp(ctx, sk_ntt=sk_ntt, pk_ntt=pk_ntt)
         self.ring.setUp(ctx.t.bit_length() - 1)
@@ -184,17 +191,18 @@ class PreparedFCSS:
     # -- BOB
     def prepareMasks(self, n, meta):
         _need(self.sampler is not None, 1, "prepareMasks: setUp first")
+        self._masks = self._y0 = None
         cols, p = meta.input_shape[0], self.fc.plan(meta)
         r = (self.sampler.words(n * cols) & (self.ctx.t - 1)).view(n, cols)
         cts = [self.fc.encryptInputVector(v, meta, (self.sampler.uniform(p.n_in), self.sampler.noise(p.n_in))) for v in r]
-        self._masks, self._y0, self._meta = r, None, meta
+        self._masks, self._mask_meta = r, meta
         return cts
 
     def finishMasks(self, out_cts):
         _need(self._masks is not None and len(out_cts) == self._masks.shape[0], 3, "finishMasks: #rows")
-        y0 = self._masks.new_empty((len(out_cts), self._meta.weight_shape[0]))
+        y0 = self._masks.new_empty((len(out_cts), self._mask_meta.weight_shape[0]))
         for row, ct in zip(y0, out_cts):
-            row.copy_(self.fc.decryptToVector(ct, self._meta))
+            row.copy_(self.fc.decryptToVector(ct, self._mask_meta))
         self._y0 = y0
 
     def openInput(self, x0):
@@ -209,8 +217,10 @@ class PreparedFCSS:
         """w [groups, rows, cols], int64 ring elements (values below 2^l or signed)"""
         _need(self.sampler is not None, 1, "prepareWeights: setUp first")
         _need(w.dim() == 3 and tuple(w.shape[1:]) == tuple(meta.weight_shape), 3, "prepareWeights: weight shape")
-        self.weights, self._meta = self.ring.encodeWeights(w), meta
+        self.weights = self._plain = self._s = self._offsets = None
+        weights, self._meta = self.ring.encodeWeights(w), meta
         self._plain = [self.fc.encodeWeightMatrix(m, meta) for m in (w & (self.ctx.t - 1)).contiguous()]
+        self.weights = weights
 
     def prepareRows(self, cts, offsets):
         """the ciphertexts of W_g r - s for BOB; offsets: groups + 1 integers on the host, every row in a group"""
@@ -218,6 +228,7 @@ class PreparedFCSS:
         _need(self.weights is not None, 1, "prepareRows: prepareWeights first")
         _need(len(offsets) == self.weights.groups + 1 and offsets[0] == 0 and offsets[-1] == len(cts) and
               all(a <= b for a, b in zip(offsets, offsets[1:])), 3, "prepareRows: offsets")
+        self._s = self._offsets = None
         from .hom_fc_ss import Meta
         meta = Meta(self._meta.weight_shape, self._meta.input_shape, False)    # the mask is BOB's alone
         n, N, smp, out, s = self.fc.plan(meta).n_out, self.ctx.N, self.sampler, [], []
@@ -239,5 +250,5 @@ class PreparedFCSS:
         _need(self._s is not None, 1, "online: no rows prepared that were not used")
         _need(opened.shape[0] == self._s.shape[0], 3, "online: #rows")
         y1 = self.ring.matMul(self.weights, opened, self._offsets, share1=share1, add=self._s, out=self._s)
-        self._s = None
+        self._s = self._offsets = None
         return y1

@@ -1,0 +1,87 @@
+"""CPU checks of PreparedFCSS's phases: nothing prepared for one set-up, matrix or batch of rows serves the next."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from openmm_amd.hom_fc_ss import Meta
+from openmm_amd.lib import MMHError
+from openmm_amd.ring_fc_ss import PreparedFCSS
+
+META = Meta((3, 4), (4,), True)
+
+
+def context(N=4096, t=1 << 20, q=(97, 193), device=0):
+    return SimpleNamespace(N=N, L=len(q), t=t, q=list(q), device=device)
+
+
+def sampler(ctx):
+    return SimpleNamespace(ctx=ctx)
+
+
+def ready(layer, rows=2):
+    """as after prepareMasks, finishMasks, prepareWeights and prepareRows"""
+    layer._meta = META
+    layer._masks, layer._y0 = torch.zeros((rows, 4), dtype=torch.int64), torch.zeros((rows, 3), dtype=torch.int64)
+    layer.weights, layer._plain = SimpleNamespace(groups=1, rows=3), [None]
+    layer._s, layer._offsets = torch.zeros((rows, 3), dtype=torch.int64), torch.tensor([0, rows])
+    return layer
+
+
+def code_of(call):
+    with pytest.raises(MMHError) as e:
+        call()
+    return e.value.code
+
+
+@pytest.fixture
+def layer():
+    p = PreparedFCSS()
+    p.setUp(context(), sampler(context()))
+    p.ring.encodeWeights = lambda w: SimpleNamespace(groups=w.shape[0], rows=w.shape[1])
+    p.fc.encodeWeightMatrix = lambda m, meta: None
+    return p
+
+
+x = torch.zeros((2, 4), dtype=torch.int64)
+
+
+def test_setup_drops_what_was_prepared(layer):
+    ready(layer)
+    other = context(N=8192)
+    layer.setUp(other, sampler(other))
+    assert code_of(lambda: layer.online(x, x)) == 1
+    assert code_of(lambda: layer.openInput(x)) == 1
+    assert code_of(lambda: layer.finishMasks([None, None])) == 3
+    assert code_of(lambda: layer.prepareRows([None, None], [0, 2])) == 1
+
+
+def test_new_weights_drop_prepared_rows(layer):
+    """otherwise W2 (x0 - r + x1) + s would come out, where the client holds W1 r - s"""
+    ready(layer)
+    layer.prepareWeights(torch.ones((1, 3, 4), dtype=torch.int64), META)
+    assert code_of(lambda: layer.online(x, x)) == 1
+
+
+def test_failed_preparations_leave_nothing_behind(layer):
+    ready(layer)
+
+    def fails(*a, **k):
+        raise MMHError(4, "no memory")
+
+    layer.fc.plan = lambda meta: SimpleNamespace(n_in=1, n_out=1)
+    layer.fc.matVecMul = fails
+    layer.sampler.reshare = lambda n: None
+    assert code_of(lambda: layer.prepareRows([None, None], [0, 2])) == 4
+    assert code_of(lambda: layer.online(x, x)) == 1
+    layer.sampler.words = fails
+    assert code_of(lambda: layer.prepareMasks(2, META)) == 4
+    assert code_of(lambda: layer.openInput(x)) == 1
+    layer.fc.encodeWeightMatrix = fails
+    assert code_of(lambda: layer.prepareWeights(torch.ones((1, 3, 4), dtype=torch.int64), META)) == 4
+    assert code_of(lambda: layer.prepareRows([None, None], [0, 2])) == 1
+
+
+@pytest.mark.parametrize("other", [dict(N=8192), dict(q=(97, 113)), dict(q=(97,)), dict(device=1)])
+def test_sampler_of_another_context_is_refused(other):
+    assert code_of(lambda: PreparedFCSS().setUp(context(), sampler(context(**other)))) == 7
