@@ -214,12 +214,12 @@ class PreparedFCSS:
 
     # -- ALICE
     def prepareWeights(self, w, meta):
-        """w [groups, rows, cols], int64 ring elements (values below 2^l or signed)"""
+        """w [groups, rows, cols], int8 to int64 ring elements (values below 2^l or signed)"""
         _need(self.sampler is not None, 1, "prepareWeights: setUp first")
         _need(w.dim() == 3 and tuple(w.shape[1:]) == tuple(meta.weight_shape), 3, "prepareWeights: weight shape")
         self.weights = self._plain = self._s = self._offsets = None
         weights, self._meta = self.ring.encodeWeights(w), meta
-        self._plain = [self.fc.encodeWeightMatrix(m, meta) for m in (w & (self.ctx.t - 1)).contiguous()]
+        self._plain = [self.fc.encodeWeightMatrix(m, meta) for m in (w.to(_INT64) & (self.ctx.t - 1)).contiguous()]
         self.weights = weights
 
     def prepareRows(self, cts, offsets):

@@ -85,3 +85,16 @@ def test_failed_preparations_leave_nothing_behind(layer):
 @pytest.mark.parametrize("other", [dict(N=8192), dict(q=(97, 113)), dict(q=(97,)), dict(device=1)])
 def test_sampler_of_another_context_is_refused(other):
     assert code_of(lambda: PreparedFCSS().setUp(context(), sampler(context(**other)))) == 7
+
+
+@pytest.mark.parametrize("t", [1 << 15, 1 << 30, 1 << 37])
+@pytest.mark.parametrize("dtype", [torch.int8, torch.int16, torch.int32, torch.int64])
+def test_weights_of_every_type_reach_the_encoder_as_words(dtype, t):
+    """the ciphertext half reads 64-bit words modulo t, whatever type the other half lays out"""
+    p, ctx, seen = PreparedFCSS(), context(t=t), []
+    p.setUp(ctx, sampler(ctx))
+    p.ring.encodeWeights = lambda w: SimpleNamespace(groups=w.shape[0], rows=w.shape[1])
+    p.fc.encodeWeightMatrix = lambda m, meta: seen.append(m)
+    w = torch.tensor([[[-1, 2, -3, 4], [5, -128, 127, 0], [1, 1, 1, 1]]], dtype=dtype)
+    p.prepareWeights(w, META)
+    assert seen[0].dtype == torch.int64 and seen[0].tolist() == [[v % t for v in row] for row in w[0].tolist()]
