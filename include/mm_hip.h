@@ -717,7 +717,8 @@ int mmh_bn_alice_finish(const mmh_ctx *ctx, const uint64_t *d_in_cts, const uint
  * (ring elements: congruent modulo 2^ring_bw is the same weight), as byte digits in matrix-core order on the current
  * device; weights need not be kept.  It reads the weights once to find how many digits the widest needs
  * (mmh_ring_weights_info: `digits`), allocates and waits for the stream, so it fails under stream capture.  The handle is
- * immutable: any number of streams and threads may use it, until destroy (which waits for kernels that read it). */
+ * immutable: any number of streams and threads may use it, until destroy (which waits for kernels that read it; a captured
+ * graph that names the handle must not run afterwards).  n_groups <= 32767, rows and cols < 2^30. */
 typedef struct mmh_ring_weights mmh_ring_weights;
 int mmh_ring_weights_create(const void *d_w, int elem_bytes, size_t n_groups, size_t rows, size_t cols, int ring_bw,
                             void *stream, mmh_ring_weights **out);
@@ -731,7 +732,8 @@ int mmh_ring_weights_info(const mmh_ring_weights *w, size_t *n_groups, size_t *r
  * not overlap the other inputs.  Results are reduced mod 2^ring_bw and exact.
  * d_ws (may be NULL) is scratch of ws_words words for this call alone: with the mmh_ring_matmul_workspace words small calls are
  * faster, with fewer (or none) they run without it.  The call allocates nothing and may be captured; calls on different streams
- * touch nothing in common.  Runs on the weights' device.  n_rows <= 2^19 per call, n_groups <= 32767. */
+ * touch nothing in common.  Runs on the weights' device.  n_tokens >= 1; n_rows <= 2^19 per call, and fewer than 2^23 tiles of
+ * 32 rows (of one group) by 256 outputs, else MMH_ERR_OUT_BOUND. */
 int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, size_t ldx, const uint64_t *d_x1, size_t ldx1,
                     size_t n_tokens, const int64_t *d_rows, const int64_t *d_offsets, size_t n_rows, const uint64_t *d_add,
                     size_t ldadd, uint64_t *d_out, size_t ldo, int zero_rest, uint64_t *d_ws, size_t ws_words, void *stream);

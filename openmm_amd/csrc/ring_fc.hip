@@ -27,6 +27,7 @@ struct mmh_ring_weights {
 };
 
 namespace mmh {
+constexpr size_t kRingGroups = 32767;   // row tiles, one more at most per group, are the second dimension of a grid (16 bits)
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
@@ -548,24 +549,25 @@ template <typename T>
 __global__ __launch_bounds__(256) void ring_weight_layout_kernel(const T *__restrict__ w, size_t rows, size_t cols, int bw,
                                                                  size_t out32, size_t k32, int nw, size_t n_units,
                                                                  int8_t *__restrict__ out) {
-  const size_t u = (size_t)blockIdx.x * 256 + threadIdx.x;   // (group, out32, k32, half, output): 16 columns of a row
-  if (u >= n_units) return;
-  const size_t frag = u >> 6, c = frag % k32, ot = frag / k32 % out32, g = frag / k32 / out32;
-  const size_t step = c >> 1, o = ot * 32 + (u & 31), place = (c & 1) * 32 + (u >> 5 & 1) * 16;
-  u64 t[16];
+  // u: (group, out32, k32, half, output), 16 columns of a row
+  for (size_t u = (size_t)blockIdx.x * 256 + threadIdx.x; u < n_units; u += (size_t)gridDim.x * 256) {
+    const size_t frag = u >> 6, c = frag % k32, ot = frag / k32 % out32, g = frag / k32 / out32;
+    const size_t step = c >> 1, o = ot * 32 + (u & 31), place = (c & 1) * 32 + (u >> 5 & 1) * 16;
+    u64 t[16];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const size_t piece = (place + e) & ~size_t(3);
-    const size_t k = cols < 4 ? place + e : ring_step_column((int)cols, (int)step) + ring_piece((int)cols, (int)piece) + (e & 3);
-    const bool in = o < rows && k < cols && k >= step * 64 && (cols >= 64 || k >= piece);
-    const u64 C = 0x8080808080808080ull;
-    t[e] = ((u64)(in ? ring_weight(w, (g * rows + o) * cols + k, bw) : 0) + C) ^ C;
-  }
-  for (int j = 0; j < nw; ++j) {
-    u32 d[4] = {0, 0, 0, 0};
+    for (int e = 0; e < 16; ++e) {
+      const size_t piece = (place + e) & ~size_t(3);
+      const size_t k = cols < 4 ? place + e : ring_step_column((int)cols, (int)step) + ring_piece((int)cols, (int)piece) + (e & 3);
+      const bool in = o < rows && k < cols && k >= step * 64 && (cols >= 64 || k >= piece);
+      const u64 C = 0x8080808080808080ull;
+      t[e] = ((u64)(in ? ring_weight(w, (g * rows + o) * cols + k, bw) : 0) + C) ^ C;
+    }
+    for (int j = 0; j < nw; ++j) {
+      u32 d[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < 16; ++e) d[e >> 2] |= (u32)(t[e] >> (8 * j) & 0xff) << (8 * (e & 3));
-    *reinterpret_cast<uint4 *>(out + (frag * nw + j) * 1024 + (u & 63) * 16) = make_uint4(d[0], d[1], d[2], d[3]);
+      for (int e = 0; e < 16; ++e) d[e >> 2] |= (u32)(t[e] >> (8 * j) & 0xff) << (8 * (e & 3));
+      *reinterpret_cast<uint4 *>(out + (frag * nw + j) * 1024 + (u & 63) * 16) = make_uint4(d[0], d[1], d[2], d[3]);
+    }
   }
 }
 
@@ -577,8 +579,8 @@ static void ring_launch_digits(const void *w, size_t n, int bw, int *need, hipSt
 template <typename T>
 static void ring_launch_layout(const void *w, const mmh_ring_weights *h, hipStream_t s) {
   const size_t units = h->groups * h->out32 * h->k32 * 64;
-  hipLaunchKernelGGL(ring_weight_layout_kernel<T>, dim3((unsigned)((units + 255) / 256)), dim3(256), 0, s, (const T *)w,
-                     h->rows, h->cols, h->bw, h->out32, h->k32, h->nw, units, h->d);
+  hipLaunchKernelGGL(ring_weight_layout_kernel<T>, dim3((unsigned)std::min<size_t>((units + 255) / 256, 65536)), dim3(256), 0, s,
+                     (const T *)w, h->rows, h->cols, h->bw, h->out32, h->k32, h->nw, units, h->d);
 }
 
 // Parts of k, by which few tiles fill the chip (48 x 4096 x 4096 72 -> 28 us, 200 x 4096 x 1024 72 -> 26, 64 x 1024 x 1024 23 -> 13),
@@ -597,8 +599,11 @@ static int ring_parts(size_t tiles, size_t steps, int products, size_t outputs) 
     if (time(p) < least) best = p, least = time(p);
   return best;
 }
-// up to 8 rows in all go to ring_few_kernel, whose waves must not sum more columns than fit 32 bits
-static bool ring_few(size_t n_rows, size_t cols, int nw) { return n_rows <= 8 && (cols / 64 / 16 + 1) * 64 * nw <= 131071; }
+// up to 8 rows in all go to ring_few_kernel, whose waves must not sum more columns than fit 32 bits and whose grid, 1024 lanes for
+// 16 outputs, has to stay below 2^32 lanes
+static bool ring_few(size_t n_rows, size_t rows, size_t cols, int nw) {
+  return n_rows <= 8 && (cols / 64 / 16 + 1) * 64 * nw <= 131071 && (rows + 15) / 16 < (size_t(1) << 22);
+}
 static constexpr int ring_products(int nx, int nw) { return 2 * (nx * nw - nw * (nw - 1) / 2); }   // of a 64-column step
 // 32-output tiles a wave computes.  Two halve the reads of digits from LDS, which bound the product when there are few digits,
 // and fit the registers (16 nx for the sums of each) for these; they pay when the chip has work enough: 4096 x 2048 x 2048 with
@@ -623,7 +628,7 @@ static void ring_launch_tiles(RingArgs a, hipStream_t s, int parts) {
 }
 template <int NX, int NW, bool TWO>
 static void ring_launch(RingArgs a, hipStream_t s) {
-  if (ring_few(a.n_rows, a.cols, NW)) {
+  if (ring_few(a.n_rows, a.n_out, a.cols, NW)) {
     const dim3 grid((a.n_out + 15) / 16, a.offsets ? std::min<unsigned>(a.groups, a.n_rows) : 1);
     hipLaunchKernelGGL((ring_few_kernel<NX, NW, TWO>), grid, dim3(1024), 0, s, a);
     return;
@@ -675,7 +680,7 @@ extern "C" int mmh_ring_weights_create(const void *d_w, int elem_bytes, size_t n
   MMH_REQUIRE(elem_bytes == 1 || elem_bytes == 2 || elem_bytes == 4 || elem_bytes == 8, MMH_ERR_INVALID_ARG);
   MMH_REQUIRE(ring_bw >= 2 && ring_bw <= 64, MMH_ERR_INVALID_ARG);
   MMH_REQUIRE(n_groups >= 1 && rows >= 1 && cols >= 1, MMH_ERR_DIM_MISMATCH);
-  MMH_REQUIRE(n_groups < (size_t(1) << 24) && rows < (size_t(1) << 30) && cols < (size_t(1) << 30), MMH_ERR_OUT_BOUND);
+  MMH_REQUIRE(n_groups <= kRingGroups && rows < (size_t(1) << 30) && cols < (size_t(1) << 30), MMH_ERR_OUT_BOUND);
   hipStream_t s = (hipStream_t)stream;
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
   (void)hipGetLastError();
@@ -750,9 +755,15 @@ static size_t ring_row_tiles(const mmh_ring_weights *w, size_t n_rows, bool offs
   return offsets ? n_rows / 32 + std::min(w->groups, n_rows) : (n_rows + 31) / 32;
 }
 static size_t ring_ws_words(const mmh_ring_weights *w, size_t n_rows, size_t row_tiles, bool two) {
-  if (w->cols < 4 || ring_few(n_rows, w->cols, w->nw)) return 0;
+  if (w->cols < 4 || ring_few(n_rows, w->rows, w->cols, w->nw)) return 0;
   const int parts = ring_call_parts(w->nx, w->nw, two, w->out32, row_tiles, w->k32 / 2, n_rows * w->rows);
   return parts > 1 ? parts * n_rows * w->rows : 0;
+}
+// a dimension of a grid holds fewer than 2^32 lanes: below 2^23 workgroups of the tile kernel
+static bool ring_grid_fits(const mmh_ring_weights *w, size_t n_rows, size_t row_tiles, bool two) {
+  if (w->cols < 4 || ring_few(n_rows, w->rows, w->cols, w->nw)) return true;
+  const int ot = ring_wide(w->nx, w->nw, two, w->out32, row_tiles) ? 2 : 1;
+  return row_tiles * ring_out_tiles(w->out32, ot) + 7 < (size_t(1) << 23);
 }
 }  // namespace mmh
 extern "C" int mmh_ring_matmul_workspace(const mmh_ring_weights *w, size_t n_rows, size_t *words) {
@@ -776,15 +787,17 @@ extern "C" int mmh_ring_matmul(const mmh_ring_weights *w, const uint64_t *d_x, s
   MMH_REQUIRE(ldo >= w->rows, MMH_ERR_DIM_MISMATCH);
   MMH_REQUIRE(!d_add || ldadd == 0 || ldadd >= w->rows, MMH_ERR_DIM_MISMATCH);
   // row tiles are the second dimension of a grid, which the hardware counts in 16 bits, and with the output tiles the first
-  MMH_REQUIRE(n_rows <= (size_t(1) << 19) && w->groups <= 32767, MMH_ERR_OUT_BOUND);
+  MMH_REQUIRE(n_rows <= (size_t(1) << 19), MMH_ERR_OUT_BOUND);
   MMH_REQUIRE((n_rows / 32 + w->groups + 8) * (w->out32 + 8) < (size_t(1) << 31), MMH_ERR_OUT_BOUND);
+  const size_t row_tiles = ring_row_tiles(w, n_rows, d_offsets != nullptr);
+  MMH_REQUIRE(ring_grid_fits(w, n_rows, row_tiles, d_x1 != nullptr), MMH_ERR_OUT_BOUND);
   RingArgs a;
   a.w = w->d, a.x = d_x, a.x1 = d_x1, a.add = d_add, a.rows = d_rows, a.offsets = d_offsets, a.out = d_out;
   a.ldx = ldx, a.ldx1 = ldx1, a.ldadd = ldadd, a.ldo = ldo, a.n_tokens = n_tokens, a.n_rows = n_rows;
   a.ws = nullptr, a.out_tiles = 0, a.zero_rest = zero_rest;
   a.groups = (int)w->groups, a.cols = (int)w->cols, a.n_out = (int)w->rows, a.k32 = (int)w->k32, a.out32 = (int)w->out32;
   a.mask = w->bw >= 64 ? ~u64(0) : (u64(1) << w->bw) - 1;
-  a.row_tiles = (int)ring_row_tiles(w, n_rows, d_offsets != nullptr);
+  a.row_tiles = (int)row_tiles;
   a.ws = d_ws && ws_words >= ring_ws_words(w, n_rows, a.row_tiles, d_x1 != nullptr) ? d_ws : nullptr;
   hipStream_t s = (hipStream_t)stream;
   bool ok = w->cols < 4;
