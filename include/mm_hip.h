@@ -748,7 +748,8 @@ int mmh_ring_matmul_workspace(const mmh_ring_weights *w, size_t n_rows, size_t *
  * of IEEE double operations, rounded to the nearest integer, ties to even: two parties on this library get the same bits.
  * x: word k of head h of token t at d_x[t*xs_token + h*xs_head + k]; out the same way with os_*, every row of its own
  * (os_token, os_head >= head_dim where there is more than one).  d_out may be d_x with the same strides, else they must not
- * overlap.  frac_bits <= 24, 0 < amplitude <= 16, head_dim <= 4096, n_heads <= 65536. */
+ * overlap.  frac_bits <= 24, 0 < amplitude <= 16, head_dim <= 4096, n_heads <= 65536; n_tokens < 2^24 whatever the heads (more
+ * where a workgroup takes several tokens of small heads; MMH_ERR_OUT_BOUND else). */
 int mmh_rotary(const uint64_t *d_x, size_t xs_token, size_t xs_head, size_t n_tokens, size_t n_heads, size_t head_dim,
                const int64_t *d_pos, const uint64_t *d_phase, size_t rot_dim, int interleaved, double amplitude, int frac_bits,
                int ring_bw, uint64_t *d_out, size_t os_token, size_t os_head, void *stream);

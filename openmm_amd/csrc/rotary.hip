@@ -157,6 +157,8 @@ static int rotary_call(const uint64_t *d_x, size_t xs_token, size_t xs_head, siz
   a.scale = amplitude * (double)(u64(1) << frac_bits);
   a.mask = bw_mask_host(bw), a.offset = offset, a.cmp_flip = cmp_flip;
   rotary_blocks(n_tokens, n_heads, head_dim, a.half, a.tokens_per_block, a.heads_per_block);
+  // a dimension of a grid holds fewer than 2^32 lanes
+  MMH_REQUIRE((n_tokens + a.tokens_per_block - 1) / a.tokens_per_block < (size_t(1) << 24), MMH_ERR_OUT_BOUND);
   const dim3 grid((unsigned)((n_tokens + a.tokens_per_block - 1) / a.tokens_per_block),
                   (unsigned)((n_heads + a.heads_per_block - 1) / a.heads_per_block));
   const size_t lds = (size_t)std::max(1, a.tokens_per_block * a.half) * sizeof(int2);
