@@ -24,13 +24,14 @@ def rotary_phases(rot_dim, base=10000, linear=1, ntk=1, yarn=None):
 
     linear: positions are divided by this factor (theta_i / linear)
     ntk: the base is multiplied by ntk^(rot_dim / (rot_dim - 2)), which leaves the fastest pair and divides the slowest by ntk
-    yarn: (factor, trained_length[, slow = 1, fast = 32]): pairs that make fewer than ``slow`` turns over the trained length
-        are divided by the factor, those with more than ``fast`` are left, those between are blended linearly in the number of
-        turns.  (The usual amplitude for it is 1 + ln(factor) / 10.)"""
+    yarn: (factor, trained_length) or (factor, trained_length, slow, fast), where slow = 1 and fast = 32 if not given: pairs that
+        make fewer than ``slow`` turns over the trained length are divided by the factor, those with more than ``fast`` are
+        left, those between are blended linearly in the number of turns.  (The usual amplitude for it is 1 + ln(factor) / 10.)"""
     _need(rot_dim >= 0 and rot_dim % 2 == 0, 3, "rotary_phases: rot_dim")
     _need(base > 0 and linear > 0 and ntk > 0, 7, "rotary_phases: base or factor")
     _need((linear != 1) + (ntk != 1) + (yarn is not None) <= 1, 7, "rotary_phases: one scaling at a time")
     _need(ntk == 1 or rot_dim > 2, 7, "rotary_phases: ntk needs two pairs")
+    _need(yarn is None or len(yarn) in (2, 4), 7, "rotary_phases: yarn")
     out = []
     with localcontext() as ctx:
         ctx.prec = 50
