@@ -238,21 +238,23 @@ class Truncation:
     def truncate_rotary(self, rotary, x, positions, shift, signed_arithmetic=True, apply_msb0_heuristic=True):
         """truncate() of ``rotary.rotate(x, positions)``, [tokens, heads, head_dim], with the turn and the step before the
         wrap protocol in one pass.  ``shift`` takes off the turn's frac_bits and whatever scale a product left in x."""
+        import torch
         bw, dim = rotary.ring_bw, x.numel()
         # what mmh_trunc_post asks for, before the protocol starts
         if not (1 <= shift < bw and (not apply_msb0_heuristic or shift <= bw - 3)):
             raise L.MMHError(7, "truncate_rotary: shift")
         if x.get_device() != self.device:
             raise L.MMHError(7, "truncate_rotary: x on another device than the protocol's")
-        adj, cmp = rotary.truncate_pre(self.party, x, positions, signed_arithmetic, apply_msb0_heuristic)
-        if dim == 0:
-            return adj
         if apply_msb0_heuristic:
             wrap_of = lambda a, c: self.aux.wrap(self.party, a, dim, bw)
         else:
             wrap_of = lambda a, c: self.aux.compare(self.party, c, dim, bw)
-        flat = None if cmp is None else cmp.view(-1)
-        out = self._truncate_rest(dim, adj.view(-1), flat, shift, bw, signed_arithmetic, apply_msb0_heuristic, wrap_of)
+        with torch.cuda.device(self.device):   # the turn is on x's device: the steps behind it have to be on its stream
+            adj, cmp = rotary.truncate_pre(self.party, x, positions, signed_arithmetic, apply_msb0_heuristic)
+            if dim == 0:
+                return adj
+            flat = None if cmp is None else cmp.view(-1)
+            out = self._truncate_rest(dim, adj.view(-1), flat, shift, bw, signed_arithmetic, apply_msb0_heuristic, wrap_of)
         return out.view(x.shape)
 
     # :84-151 (the sub-protocol gets msb_x, inverted on ALICE when signed, :118-127; the ideal one ignores it)
