@@ -13,6 +13,7 @@ models) go through one call, and which row belongs to which expert is public.  S
 classes.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -20,7 +21,7 @@ from . import lib as L
 
 
 _INT64 = torch.int64
-_stream_of = torch._C._cuda_getCurrentRawStream
+_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _need(cond, code, what):
@@ -156,6 +157,18 @@ class RingFCSS:
         return out
 
 
+def _on_its_device(method):
+    """HomFCSS and the samplers work on the current device's stream, so the layer makes its context's device the current one"""
+    @functools.wraps(method)
+    def call(self, *args, **kwargs):
+        dev = None if self.sampler is None else self.ctx.device
+        if dev is None or dev == (_current_device() if torch.cuda.is_initialized() else 0):
+            return method(self, *args, **kwargs)
+        with torch.cuda.device(dev):
+            return method(self, *args, **kwargs)
+    return call
+
+
 class PreparedFCSS:
     """An FC layer of n rows over one or more weight matrices whose ciphertext work precedes the input.  BOB:
 
@@ -189,6 +202,7 @@ class PreparedFCSS:
         return 0
 
     # -- BOB
+    @_on_its_device
     def prepareMasks(self, n, meta):
         _need(self.sampler is not None, 1, "prepareMasks: setUp first")
         self._masks = self._y0 = None
@@ -198,6 +212,7 @@ class PreparedFCSS:
         self._masks, self._mask_meta = r, meta
         return cts
 
+    @_on_its_device
     def finishMasks(self, out_cts):
         _need(self._masks is not None and len(out_cts) == self._masks.shape[0], 3, "finishMasks: #rows")
         y0 = self._masks.new_empty((len(out_cts), self._mask_meta.weight_shape[0]))
@@ -205,6 +220,7 @@ class PreparedFCSS:
             row.copy_(self.fc.decryptToVector(ct, self._mask_meta))
         self._y0 = y0
 
+    @_on_its_device
     def openInput(self, x0):
         _need(self._y0 is not None, 1, "openInput: no masks that were not used")
         _need(tuple(x0.shape) == tuple(self._masks.shape), 3, "openInput: input shape")
@@ -213,6 +229,7 @@ class PreparedFCSS:
         return opened, y0
 
     # -- ALICE
+    @_on_its_device
     def prepareWeights(self, w, meta):
         """w [groups, rows, cols], int8 to int64 ring elements (values below 2^l or signed)"""
         _need(self.sampler is not None, 1, "prepareWeights: setUp first")
@@ -222,6 +239,7 @@ class PreparedFCSS:
         self._plain = [self.fc.encodeWeightMatrix(m, meta) for m in (w.to(_INT64) & (self.ctx.t - 1)).contiguous()]
         self.weights = weights
 
+    @_on_its_device
     def prepareRows(self, cts, offsets):
         """the ciphertexts of W_g r - s for BOB; offsets: groups + 1 integers on the host, every row in a group"""
         offsets = [int(v) for v in offsets]
@@ -246,6 +264,7 @@ class PreparedFCSS:
         self._offsets = torch.tensor(offsets, dtype=_INT64, device=f"cuda:{dev}")
         return out
 
+    @_on_its_device
     def online(self, opened, share1):
         _need(self._s is not None, 1, "online: no rows prepared that were not used")
         _need(opened.shape[0] == self._s.shape[0], 3, "online: #rows")

@@ -98,3 +98,38 @@ def test_weights_of_every_type_reach_the_encoder_as_words(dtype, t):
     w = torch.tensor([[[-1, 2, -3, 4], [5, -128, 127, 0], [1, 1, 1, 1]]], dtype=dtype)
     p.prepareWeights(w, META)
     assert seen[0].dtype == torch.int64 and seen[0].tolist() == [[v % t for v in row] for row in w[0].tolist()]
+
+
+def test_every_step_makes_the_layers_device_current(monkeypatch):
+    """draws, ciphertext work and its verdicts go to the current device's stream: that has to be the context's device"""
+    current = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *a):
+            current.pop()
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    p, ctx, seen = PreparedFCSS(), context(device=1), []
+    p.setUp(ctx, sampler(ctx))
+    ready(p)
+
+    def stop(name):
+        def call(*a, **k):
+            seen.append((name, current[-1]))
+            raise MMHError(8, name)
+        return call
+
+    p._mask_meta, p.sampler.words = META, stop("words")
+    p.fc.plan, p.fc.decryptToVector, p.ring.encodeWeights = (lambda meta: SimpleNamespace(n_in=1, n_out=1)), stop("decrypt"), stop("encode")
+    p.fc.matVecMul, p.sampler.reshare, p.ring.matMul = stop("matVecMul"), lambda n: None, stop("matMul")
+    rows = [None, None]
+    for call in (lambda: p.finishMasks(rows), lambda: p.online(x, x), lambda: p.prepareRows(rows, [0, 2]), lambda: p.prepareMasks(2, META),
+                 lambda: p.prepareWeights(torch.ones((1, 3, 4), dtype=torch.int64), META)):
+        assert code_of(call) == 8
+    assert seen == [("decrypt", 1), ("matMul", 1), ("matVecMul", 1), ("words", 1), ("encode", 1)] and current == [0]
