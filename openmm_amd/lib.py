@@ -272,6 +272,42 @@ def dptr(t):
     return _vp(t.data_ptr())
 
 
+def rows_overlap(a, b):
+    """whether two sets of rows of 64-bit words share a word.  a, b: (address, words per row, ((count, stride in words), ...))"""
+    def span(p, width, dims):
+        return p, p + 8 * (width + sum((n - 1) * s for n, s in dims))
+
+    (pa, wa, da), (pb, wb, db) = a, b
+    if any(n == 0 for n, _ in da + db) or not (wa and wb):
+        return False
+    (a0, a1), (b0, b1) = span(*a), span(*b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    def merged(width, dims):     # rows that follow one another are one longer row
+        dims = sorted(((n, s) for n, s in dims if n > 1 and s), key=lambda v: v[1])
+        while dims and dims[0][1] == width:
+            width *= dims.pop(0)[0]
+        return width, dims
+
+    (wa, da), (wb, db) = merged(wa, da), merged(wb, db)
+    d = (pb - pa) // 8     # row j of b and row i of a share a word when -wb < d + start_j - start_i < wa
+    if len(da) <= 1 and len(db) <= 1 and not (da and db and da[0][1] != db[0][1]):
+        # one stride: start_j - start_i is a multiple of it, the one at -d or the next one below
+        (na, s), (nb, _) = da[0] if da else (1, (db or ((1, 1),))[0][1]), db[0] if db else (1, 0)
+        k = -d // s
+        return any(-wb < d + m * s < wa for m in (min(max(k, 1 - na), nb - 1), min(max(k + 1, 1 - na), nb - 1)))
+
+    def starts(dims, at):
+        t = np.array([at], dtype=np.int64)
+        for n, s in dims:
+            t = (t[:, None] + np.arange(n, dtype=np.int64) * s).reshape(-1)
+        return t
+
+    t, u = np.sort(starts(db, d)), starts(da, 0)
+    i = np.searchsorted(t, u + wa) - 1     # the last row of b that starts before this row of a ends
+    return bool(((i >= 0) & (t[np.maximum(i, 0)] + wb > u)).any())
+
+
 def to_device(arr, device="cuda:0"):
     """numpy uint64 array -> torch int64 CUDA tensor with the same bits."""
     import torch

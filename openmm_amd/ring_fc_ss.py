@@ -112,7 +112,8 @@ class RingFCSS:
 
         x, share1 [tokens, cols]; rows int64 [n] (None: row r reads token r); offsets int64 [groups + 1] on the device (None
         with one group); add [n, w.rows] or [w.rows]; out [n, w.rows] (a new tensor with zeros in rows of no group
-        when None).  2-D operands may have any row stride.  add may be out."""
+        when None).  2-D operands may have any row stride of a row or more, and all but out a stride of 0.  add may be out;
+        otherwise out shares no word with the other operands."""
         if self.ring_bw is None:
             raise L.MMHError(1, "matMul: setUp first")
         if not isinstance(weights, RingWeights) or not weights.handle or weights.ring_bw != self.ring_bw:
@@ -146,11 +147,19 @@ class RingFCSS:
             _need(out.shape[0] == n, 3, "matMul: out")
         if n == 0:
             return out
+        px = x.data_ptr()
+        if not new:
+            po = out.data_ptr()
+            end = po + 8 * ((n - 1) * ldo + wide)
+            for p, ld, count, width in ((px, ldx, tokens, cols), (px1, ldx1, tokens, cols), (prows, 0, 1, n),
+                                        (poff, 0, 1, weights.groups + 1), (padd, ldadd, n, wide)):
+                if p < end and po < p + 8 * ((count - 1) * ld + width) and not (p == padd == po and (ld == ldo or n == 1)):
+                    _need(not L.rows_overlap((po, wide, ((n, ldo),)), (p, width, ((count, ld),))), 7, "matMul: out overlaps an operand")
         words = weights.workspace(n)
         if words:
             ws = x.new_empty(words)
             pws = ws.data_ptr()
-        rc = weights.lib.mmh_ring_matmul(weights.handle, x.data_ptr(), ldx, px1, ldx1, tokens, prows, poff, n, padd, ldadd,
+        rc = weights.lib.mmh_ring_matmul(weights.handle, px, ldx, px1, ldx1, tokens, prows, poff, n, padd, ldadd,
                                          out.data_ptr(), ldo, new, pws, words, _stream_of(dev))
         if rc:
             L.check(rc)

@@ -1,0 +1,85 @@
+"""CPU checks of which results of a ring product or a turn are refused because they lie on top of an operand: workgroups read
+operands while others write, so such a call has no defined result."""
+import random
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from openmm_amd.lib import MMHError, rows_overlap
+from openmm_amd import ring_fc_ss
+
+WORD = 8
+
+
+def test_rows_overlap_against_sets_of_words():
+    rng, seen = random.Random(1), [0, 0]
+
+    def words(p, width, dims):
+        at = [p // WORD]
+        for n, s in dims:
+            at = [v + i * s for v in at for i in range(n)]
+        return {v + k for v in at for k in range(width)}
+
+    for _ in range(20000):
+        depth = rng.choice([1, 1, 1, 2])
+        one = lambda: (WORD * rng.randint(0, 60), rng.randint(rng.random() > 0.05, 6),
+                       tuple((rng.randint(rng.random() > 0.03, 5), rng.choice([0, 1, 3, 7, 8, 10, 20])) for _ in range(depth)))
+        a, b = one(), one()
+        if rng.random() < 0.5:
+            b = (b[0], b[1], tuple((n, s) for (n, _), (_, s) in zip(b[2], a[2])))
+        want = bool(words(*a) & words(*b))
+        seen[want] += 1
+        assert rows_overlap(a, b) == want, (a, b)
+    assert min(seen) > 1000
+
+
+@pytest.fixture
+def call(monkeypatch):
+    """matMul on host tensors: returns what it would have launched"""
+    launched = []
+    w = ring_fc_ss.RingWeights.__new__(ring_fc_ss.RingWeights)
+    w.handle, w.ring_bw, w.device, w.groups, w.rows, w.cols, w._words = 1, 64, -1, 1, 6, 6, {n: 0 for n in range(100)}
+    w.lib = SimpleNamespace(mmh_ring_matmul=lambda *a: launched.append(a) or 0, mmh_ring_weights_destroy=lambda h: 0)
+    monkeypatch.setattr(ring_fc_ss, "_stream_of", lambda dev: 0)
+    f = ring_fc_ss.RingFCSS()
+    f.setUp(64)
+
+    def run(*args, **kwargs):
+        launched.clear()
+        f.matMul(w, *args, **kwargs)
+        assert len(launched) == 1
+    return run
+
+
+def z(*shape):
+    return torch.zeros(shape, dtype=torch.int64)
+
+
+def test_product_results_beside_their_operands_are_taken(call):
+    x, wide = z(5, 6), z(5, 24)
+    call(x, out=z(5, 6))
+    call(wide[:, :6], share1=wide[:, 6:12], add=wide[:, 12:18], out=wide[:, 18:])
+    call(wide[:, :6], add=wide[:, 6:12], out=wide[:, 6:12])      # add is out
+    buf = z(10, 6)
+    call(buf[:5], out=buf[5:], offsets=z(2), rows=z(5))
+    call(buf[:5], add=buf[7], out=buf[:0].new_zeros(5, 6))
+    call(buf[:1], add=buf[1], out=buf[1:2])                      # one row: the same as add is out
+    call(buf[:1], add=buf[1:2], out=buf[1:2])
+
+
+def test_product_results_on_top_of_operands_are_refused(call):
+    x, buf, flat = z(5, 6), z(12, 6), z(400)
+    bad = [
+        lambda: call(x, out=x), lambda: call(buf[:5], out=buf[4:9]), lambda: call(x, share1=buf[:5], out=buf[3:8]),
+        lambda: call(x, add=buf[:5], out=buf[1:6]),                                       # rows above: read and written by others
+        lambda: call(x, add=buf[2], out=buf[:5]),                                         # one row for all
+        lambda: call(x, add=flat[:60].view(5, 12)[:, :6], out=flat[:40].view(5, 8)[:, :6]),
+        lambda: call(flat[:60].view(5, 12)[:, :6], out=flat[5:65].view(5, 12)[:, :6]),
+        lambda: call(x, rows=flat[3:8], out=flat[:30].view(5, 6)), lambda: call(x, offsets=flat[28:30], out=flat[:30].view(5, 6)),
+    ]
+    for i, b in enumerate(bad):
+        with pytest.raises(MMHError) as e:
+            b()
+            pytest.fail(f"case {i} was accepted")
+        assert e.value.code == 7, i
