@@ -90,6 +90,18 @@ class Rotary:
             raise L.MMHError(3, "Rotary: #positions")
         return (x.data_ptr(), token, head, tokens, heads, dim, positions.data_ptr()) + self._pairs
 
+    def _check_apart(self, out, token, head, args):
+        px, xt, xh, tokens, heads, dim, pos, phase, rot = args[:9]
+        po = out.data_ptr()
+        if not (tokens and heads):
+            return
+        end = po + 8 * ((tokens - 1) * token + (heads - 1) * head + dim)
+        mine = (po, dim, ((tokens, token), (heads, head)))
+        same = px == po and (xt == token or tokens == 1) and (xh == head or heads == 1)
+        for p, t, h, n, m, width in ((px, xt, xh, tokens, heads, dim), (pos, 0, 0, 1, 1, tokens), (phase, 0, 0, 1, 1, rot // 2)):
+            if p < end and po < p + 8 * ((n - 1) * t + (m - 1) * h + width) and not (p == px and same):
+                _need(not L.rows_overlap(mine, (p, width, ((n, t), (m, h)))), 7, "Rotary: out overlaps an operand")
+
     def _call(self, fn, args):
         args += (_stream_of(self._dev),)
         if _current_device() == self._dev:
@@ -101,7 +113,8 @@ class Rotary:
             L.check(rc)
 
     def rotate(self, x, positions, out=None):
-        """the turned share, scaled by 2^frac_bits; ``out`` may be x (same strides), or another tensor of the shape"""
+        """the turned share, scaled by 2^frac_bits; ``out`` may be x (same strides), or another tensor of the shape that shares
+        no word with x, positions or phases"""
         args = self._args(x, positions)
         if out is None:
             out = x.new_empty(x.shape)
@@ -109,6 +122,7 @@ class Rotary:
         else:
             token, head = self._strides(out)
             _need(out.shape == x.shape, 3, "Rotary: out")
+            self._check_apart(out, token, head, args)
         self._call(self.lib.mmh_rotary, args + (out.data_ptr(), token, head))
         return out
 

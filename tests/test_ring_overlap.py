@@ -83,3 +83,50 @@ def test_product_results_on_top_of_operands_are_refused(call):
             b()
             pytest.fail(f"case {i} was accepted")
         assert e.value.code == 7, i
+
+
+@pytest.fixture
+def turn(monkeypatch):
+    """rotate on host tensors of heads of 4 words: returns what it would have launched"""
+    from openmm_amd import rotary
+    launched = []
+    r = rotary.Rotary.__new__(rotary.Rotary)
+    r.head_dim, r._dev, r.phases = 4, -1, z(2)
+    r._pairs = (r.phases.data_ptr(), 4, False, 1.0, 12, 64)
+    r.lib = SimpleNamespace(mmh_rotary=None)
+    r._call = lambda fn, args: launched.append(args)
+
+    def run(x, positions, out):
+        launched.clear()
+        r.rotate(x, positions, out=out)
+        assert len(launched) == 1
+    run.phases = r.phases
+    return run
+
+
+def test_turns_beside_their_operands_are_taken(turn):
+    x, wide, pos = z(5, 3, 4), z(5, 9, 4), z(5)
+    turn(x, pos, z(5, 3, 4))
+    turn(x, pos, x)
+    turn(wide[:, :3], pos, wide[:, :3])
+    turn(wide[:, :3], pos, wide[:, 3:6])
+    turn(wide[:, ::2][:, :3], pos, wide[:, 1::2][:, :3])          # heads of two turns between one another
+    turn(wide[:, 0:1], pos, wide[:, 8:9])
+    turn(x.expand(5, 3, 4)[:1].expand(5, 3, 4), pos, z(5, 3, 4))  # one token for all
+    turn(x[:0], pos[:0], x[:0])
+
+
+def test_turns_on_top_of_operands_are_refused(turn):
+    wide, flat, pos = z(5, 9, 4), z(200), z(5)
+    bad = [
+        lambda: turn(wide[:, :3], pos, wide[:, 2:5]), lambda: turn(wide[:4, :3], pos[:4], wide[1:, :3]),
+        lambda: turn(flat[:60].view(5, 3, 4), pos, flat[1:61].view(5, 3, 4)),
+        lambda: turn(flat[:60].view(5, 3, 4), pos, flat[:60].view(3, 5, 4).transpose(0, 1)),     # the same words in another order
+        lambda: turn(wide[:1, :3].expand(5, 3, 4), pos, wide[:, :3]),
+        lambda: turn(wide[:, :3], flat[30:35], flat[:60].view(5, 3, 4)),
+    ]
+    for i, b in enumerate(bad):
+        with pytest.raises(MMHError) as e:
+            b()
+            pytest.fail(f"case {i} was accepted")
+        assert e.value.code == 7, i
