@@ -71,8 +71,9 @@ class HomFCSS:
         self._need(self.ctx is not None and self.sk_ntt is not None, 1, "encryptInputVector: no secret key")
         self._need(tuple(vec.shape) == tuple(meta.input_shape), 3, "encryptInputVector: input shape")
         p, (a, e) = self.plan(meta), rand
-        self._need(a.numel() == p.n_in * self.ctx.L * self.ctx.N and e.numel() == p.n_in * self.ctx.N, 3,
-                   "encryptInputVector: rand shape")
+        L_, N = self.ctx.L, self.ctx.N   # more polynomials than the call takes are left unread
+        self._need(a.numel() >= p.n_in * L_ * N and (a.dim() != 3 or tuple(a.shape[1:]) == (L_, N)) and
+                   e.numel() >= p.n_in * N and (e.dim() != 2 or e.shape[1] == N), 3, "encryptInputVector: rand shape")
         self._words("encryptInputVector", vec, a, e)
         out = self.ctx._empty(p.n_in, 2, self.ctx.L, self.ctx.N)
         L.check(self.ctx.lib.mmh_fc_encrypt_input(p.handle, L.dptr(self.sk_ntt), L.dptr(vec), L.dptr(a), L.dptr(e),

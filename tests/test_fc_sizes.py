@@ -68,3 +68,14 @@ def test_short_operands_are_refused(fc):
             call()
             pytest.fail(f"case {i} was accepted")
         assert e.value.code == code, i
+
+
+def test_more_randomness_than_a_call_takes_is_accepted(fc):
+    """a caller may draw for its largest layer once, in any shape that holds the words in order"""
+    for a, e in ((z(5, L, N), z(3, N)), (z(2 * L * N), z(2 * N)), (z(2 * L, N), z(2, 1, N))):
+        with pytest.raises(AssertionError, match="was reached"):
+            fc.encryptInputVector(z(16), META, (a, e))
+    for a, e in ((z(5, L, 2 * N), z(3, N)), (z(5, L, N), z(3, 2 * N)), (z(5, 1, N), z(3, N))):      # of another context
+        with pytest.raises(MMHError) as err:
+            fc.encryptInputVector(z(16), META, (a, e))
+        assert err.value.code == 3
