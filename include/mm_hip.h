@@ -715,10 +715,11 @@ int mmh_bn_alice_finish(const mmh_ctx *ctx, const uint64_t *d_in_cts, const uint
  *
  * mmh_ring_weights_create lays out d_w [n_groups][rows][cols], contiguous signed integers of elem_bytes 1, 2, 4 or 8
  * (ring elements: congruent modulo 2^ring_bw is the same weight), as byte digits in matrix-core order on the current
- * device; weights need not be kept.  It reads the weights once to find how many digits the widest needs
- * (mmh_ring_weights_info: `digits`), allocates and waits for the stream, so it fails under stream capture.  The handle is
- * immutable: any number of streams and threads may use it, until destroy (which waits for kernels that read it; a captured
- * graph that names the handle must not run afterwards).  n_groups <= 32767, rows and cols < 2^30. */
+ * device; weights need not be kept.  It reads the weights once to find how many digits the widest of all groups needs
+ * (mmh_ring_weights_info: `digits`; memory and time of a product go by it), allocates and waits for the stream, so it fails
+ * under stream capture.  The handle is immutable: any number of streams and threads may use it, until destroy (which waits for
+ * kernels that read it and frees, so not while a stream is captured; a captured graph that names the handle must not run
+ * afterwards).  n_groups <= 32767, rows and cols < 2^30. */
 typedef struct mmh_ring_weights mmh_ring_weights;
 int mmh_ring_weights_create(const void *d_w, int elem_bytes, size_t n_groups, size_t rows, size_t cols, int ring_bw,
                             void *stream, mmh_ring_weights **out);

@@ -4,8 +4,8 @@
 // Mathematics.  Both operands are written in balanced base-256 digits, x = sum x_i 256^i and w = sum w_j 256^j with
 // digits in [-128, 127]: with C = 0x80...80, the digits of v are the bytes of (v + C) ^ C (adding C makes every byte
 // digit + 128, the exclusive or takes the 128 off again as a signed byte).  l bits need nx = ceil(l/8) digits of x (what
-// lies above is a multiple of 2^l), a weight as many as its size asks for, found when the weights are laid out.  The
-// product modulo 2^l is then sum over s < nx of 256^s * sum_{i+j=s} x_i w_j, every inner sum an exact i8 x i8 -> i32
+// lies above is a multiple of 2^l), the weights as many as the widest of all groups asks for, found when they are laid out (one
+// 16-bit weight above 32639 makes them all three).  The product modulo 2^l is then sum over s < nx of 256^s * sum_{i+j=s} x_i w_j, every inner sum an exact i8 x i8 -> i32
 // matrix product, nx accumulators per output.  |x_i w_j| <= 2^14 and at most nw products share an accumulator, so up to
 // (2^17 - 1) / nw terms of k cannot overflow; longer k is added up in 64-bit pieces.  Everything is exact: the result does
 // not depend on the order of the sums.
@@ -231,9 +231,11 @@ __global__ __launch_bounds__(256) void ring_narrow_kernel(RingArgs a, int nw) {
 // through LDS.  Bound by latency: everything a wave needs of its first steps is asked for at once (kAhead steps), and it cuts
 // its own digits into LDS of its own, so the loop has no barrier.  16 x 16 products (v_mfma_i32_16x16x64_i8), of whose rows 8
 // stay zero: their rate does not matter here, their few registers do.  4 columns or more.
-// us by rows, 64 bits and two-byte weights, against the tile kernel with k split and its second launch:
-//   2048 -> 1001: 1 row 5.0 (11.3), 4 5.6 (11.5), 8 7.4 (11.5);  4096 -> 4096: 1 row 7.2 (15.0; 33.5 MB of digits = 4.7 TB/s),
-//   8 12.5 (15.7);  8192 -> 1024: 1 row 9.0 (19.1), 8 19.3 (18.9).  16 rows would read twice the words per workgroup.
+// us by rows, 64 bits and two-byte weights, calls back to back in a graph (a kernel trace reads 0.3 to 0.8 more), against the tile
+// kernel with k split and its second launch:
+//   2048 -> 1001: 1 row 5.0 (11.3), 4 5.5 (11.5), 8 7.4 (11.5);  4096 -> 4096: 1 row 7.4 (15.0; 33.5 MB of digits = 4.5 TB/s),
+//   8 12.4 (15.7);  8192 -> 1024: 1 row 9.0 (19.1), 8 19.3 (18.9).  16 rows would read twice the words per workgroup.
+// Eight digits of both operands with a second share spill 36 registers; no other variant spills.
 template <int NX, int NW, bool TWO>
 __global__ __launch_bounds__(1024) void ring_few_kernel(RingArgs a) {
   constexpr int W = 16, kAhead = NW <= 2 && !TWO ? 2 : 1;
@@ -605,10 +607,11 @@ static bool ring_few(size_t n_rows, size_t rows, size_t cols, int nw) {
   return n_rows <= 8 && (cols / 64 / 16 + 1) * 64 * nw <= 131071 && (rows + 15) / 16 < (size_t(1) << 22);
 }
 static constexpr int ring_products(int nx, int nw) { return 2 * (nx * nw - nw * (nw - 1) / 2); }   // of a 64-column step
-// 32-output tiles a wave computes.  Two halve the reads of digits from LDS, which bound the product when there are few digits,
-// and fit the registers (16 nx for the sums of each) for these; they pay when the chip has work enough: 4096 x 2048 x 2048 with
-// digits 4 x 1 135 -> 80 us, 4 x 2 135 -> 114, 5 x 1 121 -> 90, 6 x 1 121 -> 101, 5 x 2 155 -> 138, but 1024 rows 35 -> 39 us
-// (5 x 1), 40 -> 52 us (5 x 2).
+// 32-output tiles a wave computes.  Two halve the reads of digits from LDS, which bound the product when there are few digits;
+// their sums take 32 nx registers of a lane's 256.  4 x 1, 4 x 2 and 5 x 1 digits fit; 5 x 1 with a second share spills 2 registers,
+// 5 x 2 10 and 6 x 1 14, and all of them keep some 80 scalars in vector registers.  They pay nevertheless when the chip has work
+// enough: 4096 x 2048 x 2048 with digits 4 x 1 135 -> 80 us, 4 x 2 135 -> 114, 5 x 1 121 -> 90, 6 x 1 121 -> 101, 5 x 2 155 -> 138,
+// but 1024 rows 35 -> 39 us (5 x 1), 40 -> 52 us (5 x 2).  Of the tiles of one, 8 x 4 (8) and 8 x 8 (6) with a second share spill.
 static constexpr bool ring_wide_fits(int nx, int nw, bool two) { return nx + nw <= 6 || (!two && nx + nw <= 7 && nw <= 2); }
 static size_t ring_out_tiles(size_t out32, int ot) { return (out32 + 8 * ot - 1) / (8 * ot); }
 static bool ring_wide(int nx, int nw, bool two, size_t out32, size_t row_tiles) {

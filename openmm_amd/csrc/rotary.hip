@@ -10,9 +10,9 @@
 //
 // Bound: HBM, 8 B read and 8 B written per element (16 with the comparison's operand).  A workgroup computes the coefficients of
 // its tokens once, into LDS, and applies them to all their heads; a lane takes two neighbouring words per access where rows are
-// 16-byte aligned.  16384 tokens x 40 heads x 128: 252 us = 5.3 TB/s (a copy of as many bytes: 4.7); 2048 tokens 26 us = 6.4
-// TB/s; one token 2.4 us, of which a launch is 1.6.  Words at 8 modulo 16: 6000 x 13 x 43 12.9 us = 4.2 TB/s (x 42, aligned,
-// 10.9 us = 4.8).
+// 16-byte aligned.  Calls back to back in a graph: 16384 tokens x 40 heads x 128 252 us = 5.3 TB/s (torch's copy of as many
+// bytes: 4.7); one token 2.4 us, of which a launch is 1.6 (a kernel trace reads 3.1).  Out of the last-level cache, which holds
+// all of these: 2048 tokens 27 us = 6.3 TB/s, 6000 x 13 x 42 11.2 us = 4.7, words at 8 modulo 16, 6000 x 13 x 43, 12.8 us = 4.2.
 #include <algorithm>
 
 #include "common.hpp"

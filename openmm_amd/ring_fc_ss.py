@@ -11,6 +11,11 @@ clear and the server, which holds x1, computes its share
 so that y0 + y1 = W (x0 + x1).  ``PreparedFCSS`` is that layer for both parties; rows of several experts (adapters, clients'
 models) go through one call, and which row belongs to which expert is public.  Same ``gemini::Code`` errors as the other layer
 classes.
+
+``PreparedFCSS`` knows the rows of each matrix when it prepares them, before there is an input, so it serves adapters and clients'
+models; experts chosen by what a token holds need a protocol of their own around ``RingFCSS.matMul`` (``rows``), as do rings wider
+than a BFV context's plain modulus (below every prime of the context, 60 bits at most: l <= 59, and 48 with primes of 60 and 49
+bits).
 """
 import ctypes as C
 import functools
@@ -189,6 +194,8 @@ class PreparedFCSS:
 
     Rows offsets[g] .. offsets[g + 1] use matrix g.  A mask serves one input: a second openInput, or online, needs new masks.
     setUp, new masks, new weights and new rows each drop what was prepared before them.
+    The ciphertext work is per row: 2048 -> 1001 in the ring 2^37 about 0.05 ms for a mask, 0.11 to 0.2 ms for its product and
+    0.03 ms to decrypt it, beside 0.05 ms online for 64 rows together.
     ``exact`` keeps the noise terms the approximate re-sharing of ``HomFCSS.matVecMul`` leaves out (shares then add up exactly,
     otherwise within 1)."""
 
