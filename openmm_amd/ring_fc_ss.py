@@ -156,9 +156,11 @@ class RingFCSS:
         if not new:
             po = out.data_ptr()
             end = po + 8 * ((n - 1) * ldo + wide)
-            for p, ld, count, width in ((px, ldx, tokens, cols), (px1, ldx1, tokens, cols), (prows, 0, 1, n),
-                                        (poff, 0, 1, weights.groups + 1), (padd, ldadd, n, wide)):
-                if p < end and po < p + 8 * ((count - 1) * ld + width) and not (p == padd == po and (ld == ldo or n == 1)):
+            operands = [(px, ldx, tokens, cols), (px1, ldx1, tokens, cols), (prows, 0, 1, n), (poff, 0, 1, weights.groups + 1)]
+            if padd != po or (ldadd != ldo and n > 1):
+                operands.append((padd, ldadd, n, wide))
+            for p, ld, count, width in operands:
+                if p < end and po < p + 8 * ((count - 1) * ld + width):
                     _need(not L.rows_overlap((po, wide, ((n, ldo),)), (p, width, ((count, ld),))), 7, "matMul: out overlaps an operand")
         words = weights.workspace(n)
         if words:

@@ -97,9 +97,11 @@ class Rotary:
             return
         end = po + 8 * ((tokens - 1) * token + (heads - 1) * head + dim)
         mine = (po, dim, ((tokens, token), (heads, head)))
-        same = px == po and (xt == token or tokens == 1) and (xh == head or heads == 1)
-        for p, t, h, n, m, width in ((px, xt, xh, tokens, heads, dim), (pos, 0, 0, 1, 1, tokens), (phase, 0, 0, 1, 1, rot // 2)):
-            if p < end and po < p + 8 * ((n - 1) * t + (m - 1) * h + width) and not (p == px and same):
+        operands = [(pos, 0, 0, 1, 1, tokens), (phase, 0, 0, 1, 1, rot // 2)]
+        if not (px == po and (xt == token or tokens == 1) and (xh == head or heads == 1)):
+            operands.append((px, xt, xh, tokens, heads, dim))
+        for p, t, h, n, m, width in operands:
+            if p < end and po < p + 8 * ((n - 1) * t + (m - 1) * h + width):
                 _need(not L.rows_overlap(mine, (p, width, ((n, t), (m, h)))), 7, "Rotary: out overlaps an operand")
 
     def _call(self, fn, args):

@@ -130,3 +130,15 @@ def test_turns_on_top_of_operands_are_refused(turn):
             b()
             pytest.fail(f"case {i} was accepted")
         assert e.value.code == 7, i
+
+
+def test_one_operand_in_place_does_not_excuse_another(call, turn):
+    """the addend may be the result and x may be turned in place, but nothing else that starts at the same word"""
+    acc, x = z(5, 6), z(5, 6)
+    flat = z(60)
+    same = flat.view(5, 3, 4)
+    for bad in (lambda: call(acc, add=acc, out=acc), lambda: call(x, share1=acc, add=acc, out=acc),
+                lambda: call(x, rows=acc.view(-1)[:5], add=acc, out=acc), lambda: turn(same, flat[:5], same)):
+        with pytest.raises(MMHError) as e:
+            bad()
+        assert e.value.code == 7
