@@ -196,7 +196,7 @@ class PreparedFCSS:
 
     Rows offsets[g] .. offsets[g + 1] use matrix g.  A mask serves one input: a second openInput, or online, needs new masks.
     setUp, new masks, new weights and new rows each drop what was prepared before them.
-    The ciphertext work is per row: 2048 -> 1001 in the ring 2^37 about 0.05 ms for a mask, 0.11 to 0.2 ms for its product and
+    The ciphertext work is per row: 2048 -> 1001 in the ring 2^37 about 0.05 ms for a mask, 0.1 to 0.2 ms for its product and
     0.03 ms to decrypt it, beside 0.05 ms online for 64 rows together.
     ``exact`` keeps the noise terms the approximate re-sharing of ``HomFCSS.matVecMul`` leaves out (shares then add up exactly,
     otherwise within 1)."""
